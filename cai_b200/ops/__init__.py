@@ -30,6 +30,20 @@ def _p(t):
     return t.data_ptr() if t is not None else None
 
 
+def _need(ok, what):
+    if not ok:
+        raise KernelError(what)
+
+
+def _stream_for(what, *tensors):
+    """The stream of a call on these tensors, which have to be the current device's: a launch goes to that device's current stream."""
+    stream, device = _stream(), _current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise KernelError(f"{what}: a tensor on {t.device}, and cuda:{device} is the current device")
+    return stream
+
+
 def gemm(a, b, *, trans_a=False, trans_b=False, out=None, out_dtype=torch.bfloat16, accumulate=False,
          residual=None, alpha=1.0, sm_limit=0, seg_counts=None, seg_rows=0, seg_mode=0):
     """``C[M,N] = alpha * op(A) @ op(B)^T`` on the tcgen05 tensor cores.
@@ -168,6 +182,36 @@ def rmsnorm_bwd(x, g, rstd, dy, dx=None, dg=None, dx_accumulate=False, dg_accumu
     return dx, dg
 
 
+def add_rmsnorm_quant(x, residual, g, eps=1e-6, *, keep_y=False):
+    """RMSNorm in front of a block-scaled e4m3 product (:func:`gemm_fp8`): ``h = x + residual``, its norm ``y = h * rstd * g``, and y in e4m3 with a scale
+    for each row and 128 columns, in one pass.
+
+    ``x`` and ``residual`` are bf16 ``[rows, H]`` of any row pitch that is a multiple of 8, ``H`` a multiple of 128 up to 16384; ``g`` bf16 ``[H]``. Returns
+    ``(h, q, s, rstd, y)``: ``h`` bf16 (``x`` itself where ``residual`` is None), ``q`` e4m3 ``[rows, H]``, ``s`` f32 ``[rows, H / 128]``, ``rstd`` f32
+    ``[rows]``, ``y`` bf16, or None without ``keep_y`` (a weight gradient reads it). ``q`` is rounded once, from y in fp32. The gradients are
+    ``rmsnorm_bwd(h, g, rstd, dy, dx=dh, dx_accumulate=True)``: ``dh``, the gradient of ``h`` that comes past the norm, becomes that of x and of residual."""
+    _need(x.dtype is _BF16 and g.dtype is _BF16 and x.dim() == 2, "add_rmsnorm_quant: x is bf16 [rows, H], g bf16 [H]")
+    rows, H = x.shape
+    sx = x.stride()
+    _need(g.shape == (H,) and g.is_contiguous(), "add_rmsnorm_quant: g has one element a column")
+    _need(sx[1] == 1, "add_rmsnorm_quant: rows of x have to be contiguous")
+    ldx = sx[0] if rows > 1 else 0
+    ldr = 0
+    if residual is not None:
+        sr = residual.stride()
+        _need(residual.dtype is _BF16 and residual.shape == x.shape and sr[1] == 1, "add_rmsnorm_quant: the residual is like x")
+        ldr = sr[0] if rows > 1 else 0
+    stream = _stream_for("add_rmsnorm_quant", x, residual, g)
+    h = x.new_empty(rows, H) if residual is not None else None
+    y = x.new_empty(rows, H) if keep_y else None
+    q = x.new_empty(rows, H, dtype=torch.float8_e4m3fn)
+    s = x.new_empty(rows, H // 128, dtype=_F32)
+    rstd = x.new_empty(rows, dtype=_F32)
+    check(calls().cai_add_rmsnorm_quant(x.data_ptr(), ldx, _p(residual), ldr, g.data_ptr(), _p(h), _p(y), q.data_ptr(), s.data_ptr(), rstd.data_ptr(),
+                                        rows, H, float(eps), stream), "add_rmsnorm_quant")
+    return (x if h is None else h), q, s, rstd, y
+
+
 def rope_table(seq, hd, theta=10000.0, device="cuda"):
     t = torch.empty((seq, hd // 2, 2), device=device, dtype=torch.float32)
     check(calls().cai_rope_table(_p(t), seq, hd, float(theta), _stream()), "rope_table")
@@ -178,6 +222,37 @@ def rope_apply_(qkv, table, seq, nh, nkv, hd, inverse=False):
     T = qkv.shape[0]
     check(calls().cai_rope_apply(_p(qkv), _p(table), T, seq, nh, nkv, hd, qkv.stride(0), int(inverse), _stream()),
           "rope_apply")
+    return qkv
+
+
+def rope_freqs(hd, theta=10000.0, device="cuda"):
+    """The frequencies :func:`rope_apply_axes_` takes, ``theta ** (-i / (hd / 2))`` radians a position for pair i: f64 ``[hd / 2]``. A model with other
+    frequencies makes its own."""
+    return float(theta) ** (-torch.arange(hd // 2, device=device, dtype=torch.float64) / (hd // 2))
+
+
+def rope_apply_axes_(qkv, freqs, pos, nh, nkv, hd, sections, *, interleaved=False, inverse=False):
+    """Rotary embedding by the positions of one to four axes (time, height, width), in place on the q and k heads of a packed ``qkv`` (bf16
+    ``[T, (nh + 2 nkv) * hd]``, any row pitch that is a multiple of 8); returns ``qkv``.
+
+    Pair i of a head, its elements i and ``i + hd / 2``, is turned by ``pos[axis(i), t] * freqs[i]`` radians. ``pos`` int32 ``[axes, T]``, any values;
+    ``freqs`` f64 ``[hd / 2]`` (:func:`rope_freqs`); ``sections``: the axes' numbers of pairs, which add up to ``hd / 2``. They follow one another, or,
+    ``interleaved``, pair i belongs to axis ``i % axes`` as long as that axis has pairs left, and to axis 0 after that (refused where an axis would not
+    get its number). ``inverse`` turns back: the backward pass. ``hd`` a multiple of 16 up to 256."""
+    sections = tuple(sections)
+    axes = len(sections)
+    _need(qkv.dtype is _BF16 and qkv.dim() == 2 and qkv.stride(1) == 1, "rope_apply_axes_: qkv is bf16 [T, columns] with contiguous rows")
+    T, cols = qkv.shape
+    _need(cols >= (nh + nkv) * hd, "rope_apply_axes_: qkv holds fewer columns than its q and k heads")
+    _need(T < 2 or qkv.stride(0) >= cols, "rope_apply_axes_: rows of qkv overlap")
+    _need(1 <= axes <= 4 and pos.dtype is torch.int32 and pos.shape == (axes, T), "rope_apply_axes_: pos is int32 [axes, T], with one to four axes")
+    _need(pos.stride(1) == 1 or T < 2, "rope_apply_axes_: an axis' positions have to be contiguous")
+    _need(freqs.dtype is torch.float64 and freqs.shape == (hd // 2,) and freqs.is_contiguous(), "rope_apply_axes_: freqs is f64 [hd / 2]")
+    n = sections + (0,) * (4 - axes)
+    ld = qkv.stride(0) if T > 1 else (cols + 7) // 8 * 8
+    ldp = pos.stride(0) if axes > 1 else T
+    check(calls().cai_rope_apply_axes(qkv.data_ptr(), freqs.data_ptr(), pos.data_ptr(), ldp, T, nh, nkv, hd, ld, axes, n[0], n[1], n[2], n[3],
+                                      int(interleaved), int(inverse), _stream_for("rope_apply_axes_", qkv, freqs, pos)), "rope_apply_axes_")
     return qkv
 
 
@@ -249,6 +324,60 @@ def flash_attn_bwd(qkv, out, dout, lse, B, S, nh, nkv, hd, scale=None, dqkv=None
     check(calls().cai_flash_attn_bwd_parts(_p(qkv), _p(out), _p(dout), _p(lse), _p(delta), _p(dqkv), B, S, nh, nkv, hd,
                                          float(scale), int(parts), _stream()), "flash_attn_bwd")
     return dqkv
+
+
+def _window_pitch(what, t, B, S, cols):
+    """Row pitch of a packed [B * S, cols] bf16 tensor."""
+    _need(t.dtype is _BF16 and t.shape == (B * S, cols), f"{what}: needs bf16 [B * S, (heads + 2 kv_heads) * head_dim]")
+    st = t.stride()
+    _need(st[1] == 1 and (B * S < 2 or st[0] >= cols), f"{what}: rows have to be contiguous and apart")
+    return st[0] if B * S > 1 else cols
+
+
+def flash_attn_window_fwd(qkv, B, S, nh, nkv, hd, window, sinks=0, scale=None):
+    """Causal GQA flash attention with a window and sinks over packed ``qkv`` ``[B*S, (nh + 2 nkv) * hd]`` (bf16, any row pitch that is a multiple of 8): query i
+    sees key j if ``j <= i`` and (``j > i - window`` or ``j < sinks``). Any ``S``; ``window >= 1``, ``sinks >= 0``, head_dim 128. Returns ``out`` bf16
+    ``[B*S, nh * hd]`` and ``lse`` f32 ``[B, nh, S]``."""
+    ld = _window_pitch("flash_attn_window_fwd", qkv, B, S, (nh + 2 * nkv) * hd)
+    scale = hd ** -0.5 if scale is None else scale
+    stream = _stream_for("flash_attn_window_fwd", qkv)
+    out = qkv.new_empty(B * S, nh * hd)
+    lse = qkv.new_empty(B, nh, S, dtype=_F32)
+    check(calls().cai_flash_attn_window_fwd(qkv.data_ptr(), ld, out.data_ptr(), lse.data_ptr(), B, S, nh, nkv, hd, float(scale), window, sinks, stream),
+          "flash_attn_window_fwd")
+    return out, lse
+
+
+def flash_attn_window_bwd(qkv, out, dout, lse, B, S, nh, nkv, hd, window, sinks=0, scale=None, dqkv=None, delta=None, scratch=None):
+    """Gradient of :func:`flash_attn_window_fwd` with respect to ``qkv``, packed like it (``dqkv``, made where it is None). ``out`` and ``lse`` are the forward
+    pass's, ``dout`` the gradient of ``out``. ``delta`` (f32 ``[B, nh, S]``) and ``scratch`` (uint8, :func:`flash_attn_window_bwd_scratch` bytes) are
+    workspaces, made where they are None; calls that may overlap need their own. The same bits in every run."""
+    cols = (nh + 2 * nkv) * hd
+    ld = _window_pitch("flash_attn_window_bwd", qkv, B, S, cols)
+    for t in (out, dout):
+        _need(t.dtype is _BF16 and t.shape == (B * S, nh * hd) and t.is_contiguous(), "flash_attn_window_bwd: out and dout are bf16 [B * S, heads * head_dim]")
+    _need(lse.dtype is _F32 and lse.shape == (B, nh, S) and lse.is_contiguous(), "flash_attn_window_bwd: lse is f32 [B, heads, S]")
+    scale = hd ** -0.5 if scale is None else scale
+    stream = _stream_for("flash_attn_window_bwd", qkv, out, dout, lse, dqkv, delta, scratch)
+    if dqkv is None:
+        dqkv = qkv.new_empty(B * S, cols)
+    ldq = _window_pitch("flash_attn_window_bwd", dqkv, B, S, cols)
+    if delta is None:
+        delta = lse.new_empty(B, nh, S)
+    _need(delta.dtype is _F32 and delta.numel() >= B * nh * S and delta.is_contiguous(), "flash_attn_window_bwd: delta is f32 [B, heads, S]")
+    need = calls().cai_flash_attn_window_bwd_scratch(B, S, nh, nkv, window, sinks)
+    if scratch is None:
+        scratch = qkv.new_empty(need, dtype=torch.uint8) if need else None
+    else:
+        _need(scratch.numel() * scratch.element_size() >= need and scratch.is_contiguous(), f"flash_attn_window_bwd: the scratch has to have {need} bytes")
+    check(calls().cai_flash_attn_window_bwd(qkv.data_ptr(), ld, out.data_ptr(), dout.data_ptr(), lse.data_ptr(), delta.data_ptr(), dqkv.data_ptr(), ldq,
+                                            _p(scratch), B, S, nh, nkv, hd, float(scale), window, sinks, stream), "flash_attn_window_bwd")
+    return dqkv
+
+
+def flash_attn_window_bwd_scratch(B, S, nh, nkv, window, sinks=0):
+    """Bytes of scratch :func:`flash_attn_window_bwd` takes on the current device."""
+    return calls().cai_flash_attn_window_bwd_scratch(B, S, nh, nkv, window, sinks)
 
 
 __all__ = [n for n in dir() if not n.startswith("_")]

@@ -97,6 +97,12 @@ def _declare(L):
     if hasattr(L, "cai_flash_attn_bwd"):
         L.cai_flash_attn_bwd.argtypes = [P, P, P, P, P, P, I, I, I, I, I, F, P]
         L.cai_flash_attn_bwd_parts.argtypes = [P, P, P, P, P, P, I, I, I, I, I, F, I, P]
+    L.cai_add_rmsnorm_quant.argtypes = [P, LL, P, LL, P, P, P, P, P, P, I, I, F, P]
+    L.cai_rope_apply_axes.argtypes = [P, P, P, LL, I, I, I, I, LL, I, I, I, I, I, I, I, P]
+    L.cai_flash_attn_window_fwd.argtypes = [P, LL, P, P, I, I, I, I, I, F, I, I, P]
+    L.cai_flash_attn_window_bwd_scratch.argtypes = [I, I, I, I, I, I]
+    L.cai_flash_attn_window_bwd_scratch.restype = LL
+    L.cai_flash_attn_window_bwd.argtypes = [P, LL, P, P, P, P, P, LL, P, I, I, I, I, I, F, I, I, P]
 
 
 def check(rc: int, what: str):

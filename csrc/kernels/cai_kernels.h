@@ -166,12 +166,28 @@ CAI_API int cai_rmsnorm_dg_sums(const cai_dg_sum* sums, int n, int H, void* stre
  * written. Needs no GPU. */
 CAI_API int cai_rmsnorm_bwd_rounds(int rows, int H, int ctas, int cta, int lost_round, int* events, int capacity);
 
+/* RMSNorm in front of a block-scaled e4m3 product, with the residual's addition: h = bf16(x + residual) (residual null: h = x),
+ * rstd = (mean(h^2) + eps)^(-1/2), y = h * rstd * g, scale[row, b] = max |y| of columns 128 b .. 128 b + 127 / 448 (1 where they are all zero),
+ * q = e4m3(y / scale), rounded once. x and residual have pitches ldx and ldr (elements, multiples of 8; h may be x or residual where their pitch is H);
+ * h, y [rows, H] bf16 (either may be null), q [rows, H] e4m3, scale [rows, H / 128] and rstd [rows] f32. H % 128 == 0, H <= 16384, every row on 16
+ * bytes. The backward pass is cai_rmsnorm_bwd on h with dx_accumulate: dx holds the gradient of h that comes past the norm, and ends as that of
+ * x and of the residual. No counterpart in the reference. */
+CAI_API int cai_add_rmsnorm_quant(const void* x, long long ldx, const void* residual, long long ldr, const void* g, void* h, void* y, void* q,
+                                  float* scale, float* rstd, int rows, int H, float eps, void* stream);
+
 /* ---- rotary embedding, in place on the q and k heads of a packed [T, (nh+2*nkv)*hd] buffer.
  * table is float2 [seq, hd/2] (cos, sin); position of row t is t % seq. inverse=1 applies the
  * transpose rotation (backward). */
 CAI_API int cai_rope_table(float* table, int seq, int hd, float theta, void* stream);
 CAI_API int cai_rope_apply(void* qkv, const float* table, int T, int seq, int nh, int nkv, int hd,
                            long long ld, int inverse, void* stream);
+
+/* The same by the positions of `axes` (1 to 4) axes: pair i of a head, its elements i and i + hd / 2, is turned by
+ * pos[axis(i) * ldp + row] * freqs[i] radians (any int; the product is taken in 64 bits). axis(i): the first n0 pairs belong to axis 0, the next n1 to axis 1
+ * and so on (the rest of the n are 0); interleaved, pair i belongs to axis i % axes while i / axes < n of that axis, and to axis 0 otherwise
+ * (refused where an axis would not get its n). n0 + n1 + n2 + n3 = hd / 2, hd a multiple of 16 up to 256. */
+CAI_API int cai_rope_apply_axes(void* qkv, const double* freqs, const int* pos, long long ldp, int T, int nh, int nkv, int hd, long long ld, int axes,
+                                int n0, int n1, int n2, int n3, int interleaved, int inverse, void* stream);
 
 /* ---- SwiGLU on a packed [T, 2F] gate|up buffer (reference: src/cuda/cai_kernels.cu:146-160) */
 CAI_API int cai_swiglu_fwd(const void* gu, void* act, int T, int F, void* stream);
@@ -246,4 +262,23 @@ CAI_API int cai_flash_attn_bwd_parts(const void* qkv, const void* out, const voi
  * bit, without the pass. */
 CAI_API int cai_flash_attn_bwd_rope(const void* qkv, const void* out, const void* dout, const float* lse, float* delta, void* dqkv,
                                     const float* table, int B, int S, int nh, int nkv, int hd, float scale, int parts, void* stream);
+
+/* ---- the same with a window and sinks, over sequences of any length: query i sees key j if j <= i and (j > i - window or j < sinks). window >= 1, so
+ * that every row sees itself; sinks >= 0. qkv and dqkv have row pitches ld and ldq (multiples of 8 elements); out, dout [B*S, nh*hd] and lse, delta
+ * [B, nh, S] are dense. Rows of 16-byte alignment, head_dim 128. Nothing is read or written past a sequence's last row. Values have to be finite: a
+ * hidden key has weight 0, and 0 times what is not finite is not 0. */
+CAI_API int cai_flash_attn_window_fwd(const void* qkv, long long ld, void* out, float* lse, int B, int S, int nh, int nkv, int hd, float scale,
+                                      int window, int sinks, void* stream);
+/* Gradients of all q, k and v heads, the same bits in every run. delta: scratch f32 [B, nh, S]; scratch: as many bytes as
+ * cai_flash_attn_window_bwd_scratch says for the current device (which may be 0: sums of key tiles that several CTAs share), on 16 bytes. No other
+ * memory is shared between calls: two may overlap. */
+CAI_API long long cai_flash_attn_window_bwd_scratch(int B, int S, int nh, int nkv, int window, int sinks);
+/* What the CTAs of its dK / dV part work on, on `sms` SMs, eight ints a CTA: key tile, batch, kv head, first query head, query heads, first query tile, query
+ * tiles (none or less: nothing), slot of 128 KB of the scratch (-1: none). Returns their number, of which `capacity` are written. And the key tiles
+ * that query tile i takes, in order. Need no GPU. */
+CAI_API int cai_flash_attn_window_walk(int B, int S, int nh, int nkv, int window, int sinks, int sms, int* parts, int capacity);
+CAI_API int cai_flash_attn_window_keys(int S, int window, int sinks, int i, int* tiles, int capacity);
+CAI_API int cai_flash_attn_window_bwd(const void* qkv, long long ld, const void* out, const void* dout, const float* lse, float* delta, void* dqkv,
+                                      long long ldq, void* scratch, int B, int S, int nh, int nkv, int hd, float scale, int window, int sinks,
+                                      void* stream);
 #endif /* CAI_KERNELS_H */

@@ -47,6 +47,37 @@
 
 namespace cai {
 
+// How the dK / dV part of the windowed form is cut into CTAs. A key tile's sum runs over the query heads of its group and over the query tiles that see it: those of
+// the window, and, where it holds sinks, all later ones. The heads are cut into `head_parts`, the later query tiles into `far_parts` of
+// `far_tiles` each. Tiles with more than one part leave sums in fp32 in the caller's scratch, 128 KB a part, which a
+// second kernel adds up in a fixed order.
+struct AttnWindowParts {
+    int head_parts, far_parts, far_tiles;
+    int sink_tiles;          // key tiles that hold sinks and are seen by query tiles behind their window
+    int near_ctas, far_ctas, near_slots;
+};
+
+// The part that CTA `lin` of the dK / dV part works on: those of the window first, key tiles slowest, heads and batch fastest.
+struct WindowPart {
+    int j, b, g, h_first, heads;    // key tile, batch, kv head, query heads
+    int q_first, q_tiles;           // query tiles of each head (none or less: nothing to do, for the last far part of a late tile)
+    int slot;                       // of the scratch; -1: the CTA has the whole sum
+    __host__ __device__ WindowPart(const AttnWindow& w, const AttnWindowParts& c, int B, int S, int nh, int nkv, int lin) {
+        const int rep = nh / nkv, nq = (S + kAttnTile - 1) / kAttnTile, stride = nkv * c.head_parts * B;
+        const bool far = lin >= c.near_ctas;
+        const int rest = (far ? lin - c.near_ctas : lin) / stride, at = lin % stride, y = at % (nkv * c.head_parts);   // near_ctas is a multiple of stride
+        j = far ? rest / c.far_parts : rest;
+        b = at / (nkv * c.head_parts);
+        g = y / c.head_parts;
+        heads = rep / c.head_parts;
+        h_first = g * rep + y % c.head_parts * heads;
+        const int near_end = window_last_query_tile(w, j, nq) + 1;
+        q_first = far ? near_end + rest % c.far_parts * c.far_tiles : j;
+        q_tiles = (far && q_first + c.far_tiles < nq ? q_first + c.far_tiles : far ? nq : near_end) - q_first;
+        slot = c.head_parts == 1 && (j >= c.sink_tiles || near_end >= nq) ? -1 : far ? c.near_slots + lin - c.near_ctas : lin;
+    }
+};
+
 struct AttnBwdParams {
     int B, S, nh, nkv;
     float scale, scale_log2;
@@ -59,6 +90,10 @@ struct AttnBwdParams {
     int split_heads;
     unsigned int* chain;
     const float2* rope;          // (cos, sin) [S][64]: dQ and dK leave rotated back (null: as they are)
+    AttnWindow win;              // of the windowed form
+    AttnWindowParts cut;
+    float* partial;
+    long long ldq;               // row pitch of dqkv
 };
 
 // chain counters of the head-split dK / dV kernel: one per (batch, kv group, kv tile).
@@ -143,8 +178,10 @@ __device__ __forceinline__ void stage_acc_chunk(uint32_t tacc, uint32_t stage, i
 // A thread of 512 takes kPieces times eight columns and the eight that are 64 further on: item `first` of eight a row, 128 rows a tile of 64 KB, then
 // every 512th. Tile t leaves at dst[t], times mul[t]; where `rope` is given (the row of its table that belongs to row 0), tile 0 is rounded, as it
 // would be in memory, and rotated back.
-template <bool kAdd, int kPieces>
-__device__ __forceinline__ void write_staged(uint32_t stage, __nv_bfloat16* const (&dst)[2], const float (&mul)[2], long long ld, int first, const float2* rope) {
+// kCut: only the tiles' first `rows` rows are there.
+template <bool kAdd, int kPieces, bool kCut = false>
+__device__ __forceinline__ void write_staged(uint32_t stage, __nv_bfloat16* const (&dst)[2], const float (&mul)[2], long long ld, int first, const float2* rope,
+                                             int rows = kAttnTile) {
     uint4 old[kPieces][2];
     if constexpr (kAdd) {
 #pragma unroll
@@ -159,6 +196,7 @@ __device__ __forceinline__ void write_staged(uint32_t stage, __nv_bfloat16* cons
     for (int i = 0; i < kPieces; ++i) {
         const int item = first + i * 512, r = (item >> 3) & 127, c = (item & 7) * 2;
         const uint32_t row = stage + (i >> 1) * 65536 + r * 512;
+        if (kCut && r >= rows) continue;
         uint32_t o[2][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -199,8 +237,9 @@ __device__ __forceinline__ void write_staged(uint32_t stage, __nv_bfloat16* cons
 
 // Probabilities of one thread's 32 score columns, in place: exp2(s * scale_log2 - lse2). In the transposed form (dK / dV)
 // a column is a query with its own lse2; in the other (dQ) the thread's row is the query. One half (16 columns) per call.
-template <bool kDiag, int kHalf>
-__device__ __forceinline__ void prob_cols(uint32_t (&v)[32], const float4 (&ls)[4], float scale_log2, int r, int qb) {
+// kWindow: this thread's key is seen by the columns from..from + span - 1.
+template <bool kDiag, int kHalf, bool kWindow = false>
+__device__ __forceinline__ void prob_cols(uint32_t (&v)[32], const float4 (&ls)[4], float scale_log2, int r, int qb, int from = 0, int span = 0) {
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
         const float l[4] = {ls[e4].x, ls[e4].y, ls[e4].z, ls[e4].w};
@@ -209,19 +248,28 @@ __device__ __forceinline__ void prob_cols(uint32_t (&v)[32], const float4 (&ls)[
             const int e = kHalf * 16 + e4 * 4 + t;
             float pv = fast_exp2(__uint_as_float(v[e]) * scale_log2 - l[t]);
             if constexpr (kDiag) {
-                if (r > qb + e) pv = 0.f;  // key (row r) may not lie after the query (column)
+                if constexpr (kWindow) {
+                    if (static_cast<unsigned>(e - from) >= static_cast<unsigned>(span)) pv = 0.f;
+                } else {
+                    if (r > qb + e) pv = 0.f;  // key (row r) may not lie after the query (column)
+                }
             }
             v[e] = __float_as_uint(pv);
         }
     }
 }
-template <bool kDiag>
-__device__ __forceinline__ void prob_rows(uint32_t (&v)[32], float lse2, float scale_log2, int r, int kb) {
+// kWindow: this thread's query sees the columns first < e <= last and those below `sink`.
+template <bool kDiag, bool kWindow = false>
+__device__ __forceinline__ void prob_rows(uint32_t (&v)[32], float lse2, float scale_log2, int r, int kb, int last = 0, int first = 0, int sink = 0) {
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
         float pv = fast_exp2(__uint_as_float(v[e]) * scale_log2 - lse2);
         if constexpr (kDiag) {
-            if (kb + e > r) pv = 0.f;
+            if constexpr (kWindow) {
+                if (e > last || (e <= first && e >= sink)) pv = 0.f;
+            } else {
+                if (kb + e > r) pv = 0.f;
+            }
         }
         v[e] = __float_as_uint(pv);
     }
@@ -242,8 +290,21 @@ __device__ __forceinline__ void issue_pd_ss(uint32_t d_tmem, uint64_t a_desc, ui
                     (accumulate || k > 0) ? 1u : 0u);
 }
 
+// A tile of the packed activation or of dO: the windowed form has the sequences apart (rows past a sequence's end come as zeros).
+template <bool kWindow>
+__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* tm, uint64_t* bar, int x, int b, int S, int row) {
+    if constexpr (kWindow) {
+        tma_load_3d(dst, tm, bar, x, row, b);
+        tma_load_3d(static_cast<uint8_t*>(dst) + kAttnSub, tm, bar, x + 64, row, b);
+    } else {
+        tma_load_2d(dst, tm, bar, x, b * S + row);
+        tma_load_2d(static_cast<uint8_t*>(dst) + kAttnSub, tm, bar, x + 64, b * S + row);
+    }
+}
+
 // ---------------------------------------------------------------------------- dK / dV
-// One CTA's work: number `lin` of the (kv tile, batch, head) triples.
+// One CTA's work: number `lin` of the (kv tile, batch, head) triples; kWindow: of the parts of AttnWindowParts, those of the window first.
+template <bool kWindow>
 __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUtensorMap& tm_do, const AttnBwdParams& p, uint8_t* smem, int lin) {
     uint8_t* sK = smem;
     uint8_t* sV = smem + kAttnTileBytes;
@@ -270,16 +331,22 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // kv tile slowest, heaviest first; heads and batch fastest. Heads are kv groups (a CTA sweeps the group's query heads) or,
     // with split_heads, query heads
+    const WindowPart part(p.win, p.cut, p.B, p.S, p.nh, p.nkv, kWindow ? lin : 0);
     const int heads = p.split_heads ? p.nh : p.nkv, heads_all = heads * p.B;
-    const int j = lin / heads_all;  // kv tile
-    const int ysel = (lin % heads_all) % heads, b = (lin % heads_all) / heads;
+    const int j = kWindow ? part.j : lin / heads_all;  // kv tile
+    const int ysel = (lin % heads_all) % heads, b = kWindow ? part.b : (lin % heads_all) / heads;
     const int rep = p.nh / p.nkv;
-    const int g = p.split_heads ? ysel / rep : ysel;
-    const int h_first = p.split_heads ? ysel : g * rep;
-    const int turn = p.split_heads ? ysel - g * rep : 0;   // my place in the group's accumulation chain
+    const int g = kWindow ? part.g : p.split_heads ? ysel / rep : ysel;
+    const int h_first = kWindow ? part.h_first : p.split_heads ? ysel : g * rep;
+    const int turn = !kWindow && p.split_heads ? ysel - g * rep : 0;   // my place in the group's accumulation chain
     const int nq = p.S / kAttnTile;
-    const int per_head = nq - j;          // query tiles at or below the diagonal
-    const int iters = (p.split_heads ? 1 : rep) * per_head;
+    const int q_first = kWindow ? part.q_first : j;
+    const int per_head = kWindow ? part.q_tiles : nq - j;          // query tiles at or below the diagonal
+    const int iters = (kWindow ? part.heads : p.split_heads ? 1 : rep) * per_head;
+    if (kWindow && per_head <= 0) {
+        grid_dep_wait();
+        return;
+    }
     const int row_base = b * p.S;
     const int col_k = (p.nh + g) * kAttnHD, col_v = (p.nh + p.nkv + g) * kAttnHD;
 
@@ -316,28 +383,21 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
 
     if (warp == 0) {
         if (lane == 0) {
-            const int kv_row = row_base + j * kAttnTile;
             mbar_expect_tx(kv_full, 2 * kAttnTileBytes);
-            tma_load_2d(sK, &tm_qkv, kv_full, col_k, kv_row);
-            tma_load_2d(sK + kAttnSub, &tm_qkv, kv_full, col_k + 64, kv_row);
-            tma_load_2d(sV, &tm_qkv, kv_full, col_v, kv_row);
-            tma_load_2d(sV + kAttnSub, &tm_qkv, kv_full, col_v + 64, kv_row);
+            load_tile<kWindow>(sK, &tm_qkv, kv_full, col_k, b, p.S, j * kAttnTile);
+            load_tile<kWindow>(sV, &tm_qkv, kv_full, col_v, b, p.S, j * kAttnTile);
             bool ok = true;
             for (int it = 0; it < iters && ok; ++it) {
                 const int slot = it & 1;
                 const uint32_t ph = (it >> 1) & 1;
                 const int h = h_first + it / per_head;
-                const int q_row = row_base + (j + it % per_head) * kAttnTile;
+                const int q_row = (q_first + it % per_head) * kAttnTile;
                 if (!mbar_wait(&q_empty[slot], ph ^ 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
                 mbar_expect_tx(&q_full[slot], kAttnTileBytes);
-                uint8_t* q = sQ + slot * kAttnTileBytes;
-                tma_load_2d(q, &tm_qkv, &q_full[slot], h * kAttnHD, q_row);
-                tma_load_2d(q + kAttnSub, &tm_qkv, &q_full[slot], h * kAttnHD + 64, q_row);
+                load_tile<kWindow>(sQ + slot * kAttnTileBytes, &tm_qkv, &q_full[slot], h * kAttnHD, b, p.S, q_row);
                 if (!mbar_wait(&do_empty[slot], ph ^ 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
                 mbar_expect_tx(&do_full[slot], kAttnTileBytes);
-                uint8_t* d = sdO + slot * kAttnTileBytes;
-                tma_load_2d(d, &tm_do, &do_full[slot], h * kAttnHD, q_row);
-                tma_load_2d(d + kAttnSub, &tm_do, &do_full[slot], h * kAttnHD + 64, q_row);
+                load_tile<kWindow>(sdO + slot * kAttnTileBytes, &tm_do, &do_full[slot], h * kAttnHD, b, p.S, q_row);
             }
             grid_dep_launch();
             if (!ok)
@@ -418,15 +478,19 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
         const uint32_t pchunk = (grp & 1) * 4, psw = r & 7;
         bool ok = true;
         // statistics of this warp's queries (a lane holds one), fetched a step ahead; shared through the warp's own 32 words
-        auto stat_at = [&](const float* v, int it) {
+        // (past the sequence's end there is none: a probability of exp2(-inf) = 0)
+        auto stat_at = [&](const float* v, int it, float none) {
             const int h = h_first + it / per_head;
-            const int i = j + it % per_head;
+            const int i = q_first + it % per_head;
+            if (kWindow && i * kAttnTile + qb + lane >= p.S) return none;
             return v[(static_cast<long long>(b) * p.nh + h) * p.S + i * kAttnTile + qb + lane];
         };
-        float lse_next = stat_at(p.lse, 0), delta_next = stat_at(p.delta, 0);
+        float lse_next = stat_at(p.lse, 0, INFINITY), delta_next = stat_at(p.delta, 0, 0.f);
 #pragma unroll 1
         for (int it = 0; it < iters; ++it) {
-            const bool diag = it % per_head == 0;
+            const int i = q_first + it % per_head;
+            const bool diag = kWindow ? window_masks(p.win, i, j) : it % per_head == 0;
+            const int from = kWindow ? (j - i) * kAttnTile + r - qb : 0, span = !kWindow || j * kAttnTile + r < p.win.sinks ? 0x7fffffff : p.win.window;
             const float delta = delta_next;
             if (!mbar_wait_warp(s_full, it & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
             tc_fence_after();
@@ -435,8 +499,8 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
             __syncwarp();
             stat[lane] = lse_next * 1.4426950408889634f;
             if (it + 1 < iters) {
-                lse_next = stat_at(p.lse, it + 1);
-                delta_next = stat_at(p.delta, it + 1);
+                lse_next = stat_at(p.lse, it + 1, INFINITY);
+                delta_next = stat_at(p.delta, it + 1, 0.f);
             }
             __syncwarp();
             float4 ls[4];
@@ -445,11 +509,11 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
             tmem_ld_wait();
             tc_fence_before();
             mbar_arrive_warp(s_empty);
-            if (diag) prob_cols<true, 0>(pr, ls, p.scale_log2, r, qb);
+            if (diag) prob_cols<true, 0, kWindow>(pr, ls, p.scale_log2, r, qb, from, span);
             else prob_cols<false, 0>(pr, ls, p.scale_log2, r, qb);
 #pragma unroll
             for (int e = 0; e < 4; ++e) ls[e] = reinterpret_cast<const float4*>(stat)[4 + e];
-            if (diag) prob_cols<true, 1>(pr, ls, p.scale_log2, r, qb);
+            if (diag) prob_cols<true, 1, kWindow>(pr, ls, p.scale_log2, r, qb, from, span);
             else prob_cols<false, 1>(pr, ls, p.scale_log2, r, qb);
             __syncwarp();
             stat[lane] = delta;
@@ -497,13 +561,26 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
             stage_acc_chunk((grp < 2 ? tdK : tdV) + lane_bits, stage + (grp >> 1) * 65536, r, c0);
             stage_acc_chunk((grp < 2 ? tdK : tdV) + lane_bits, stage + (grp >> 1) * 65536, r, c0 + 1);
         }
+        if constexpr (kWindow) fence_proxy_async_smem();
         bar_sync_compute();
-        const long long ld = static_cast<long long>(p.nh + 2 * p.nkv) * kAttnHD;
+        if constexpr (kWindow) {
+            // a part leaves its two sums as they are staged; the kernel behind this one adds the parts up
+            if (part.slot >= 0) {
+                if (ok && threadIdx.x == 128) {
+                    char* to = reinterpret_cast<char*>(p.partial) + part.slot * 131072ll;
+                    for (int k = 0; k < 8; ++k) bulk_store(to + k * 16384, smem + k * 16384, 16384);
+                    tma_store_commit();
+                    tma_store_wait0();
+                }
+                ok = false;   // nothing else leaves
+            }
+        }
+        const long long ld = kWindow ? p.ldq : static_cast<long long>(p.nh + 2 * p.nkv) * kAttnHD;
         __nv_bfloat16* row0 = p.dqkv + (static_cast<long long>(row_base) + j * kAttnTile) * ld;
         __nv_bfloat16* const dst[2] = {row0 + col_k, row0 + col_v};
         const float mul[2] = {p.scale, 1.f};
         const int first = threadIdx.x - 128;
-        unsigned int* cnt = p.split_heads ? p.chain + (static_cast<long long>(b) * p.nkv + g) * nq + j : nullptr;
+        unsigned int* cnt = !kWindow && p.split_heads ? p.chain + (static_cast<long long>(b) * p.nkv + g) * nq + j : nullptr;
         if (turn > 0 && ok) {
             // heads of the group add in turn: wait (bounded) until the heads before me are done
             ok = false;
@@ -517,11 +594,12 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
         }
         if (ok) {
             // the last of the heads turns the finished sum
-            const float2* rope = p.rope && (!p.split_heads || turn + 1 == rep) ? p.rope + static_cast<long long>(j) * kAttnTile * 64 : nullptr;
-            if (turn == 0) write_staged<false, 4>(stage, dst, mul, ld, first, rope);
+            const float2* rope = !kWindow && p.rope && (!p.split_heads || turn + 1 == rep) ? p.rope + static_cast<long long>(j) * kAttnTile * 64 : nullptr;
+            if constexpr (kWindow) write_staged<false, 4, true>(stage, dst, mul, ld, first, nullptr, p.S - j * kAttnTile);
+            else if (turn == 0) write_staged<false, 4>(stage, dst, mul, ld, first, rope);
             else write_staged<true, 4>(stage, dst, mul, ld, first, rope);
         }
-        if (p.split_heads) {
+        if (!kWindow && p.split_heads) {
             __threadfence();
             bar_sync_compute();
             if (threadIdx.x == 128) {   // first compute thread: everyone's rows are written and fenced
@@ -539,6 +617,7 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
 }
 
 // ---------------------------------------------------------------------------- dQ
+template <bool kWindow>
 __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtensorMap& tm_do, const AttnBwdParams& p, uint8_t* smem, int lin) {
     uint8_t* sQ = smem;
     uint8_t* sdO = smem + kAttnTileBytes;
@@ -560,10 +639,11 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int heads_all = p.nh * p.B;
-    const int i = p.S / kAttnTile - 1 - lin / heads_all;  // q tile, heaviest first across all heads
+    const int i = (p.S + kAttnTile - 1) / kAttnTile - 1 - lin / heads_all;  // q tile, heaviest first across all heads
     const int h = (lin % heads_all) % p.nh, b = (lin % heads_all) / p.nh;
     const int g = h / (p.nh / p.nkv);
-    const int n = i + 1;
+    const WindowKeys keys(p.win, i);
+    const int n = kWindow ? keys.n : i + 1;
     const int row_base = b * p.S;
     const int col_q = h * kAttnHD, col_k = (p.nh + g) * kAttnHD, col_v = (p.nh + p.nkv + g) * kAttnHD;
 
@@ -600,29 +680,22 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
 
     if (warp == 0) {
         if (lane == 0) {
-            const int q_row = row_base + i * kAttnTile;
             mbar_expect_tx(q_full, 2 * kAttnTileBytes);
-            tma_load_2d(sQ, &tm_qkv, q_full, col_q, q_row);
-            tma_load_2d(sQ + kAttnSub, &tm_qkv, q_full, col_q + 64, q_row);
-            tma_load_2d(sdO, &tm_do, q_full, col_q, q_row);
-            tma_load_2d(sdO + kAttnSub, &tm_do, q_full, col_q + 64, q_row);
+            load_tile<kWindow>(sQ, &tm_qkv, q_full, col_q, b, p.S, i * kAttnTile);
+            load_tile<kWindow>(sdO, &tm_do, q_full, col_q, b, p.S, i * kAttnTile);
             bool ok = true;
             int ks = 0;
             uint32_t kph = 0;
             for (int j = 0; j < n && ok; ++j) {
                 const int slot = j & 1;
                 const uint32_t ph = (j >> 1) & 1;
-                const int kv_row = row_base + j * kAttnTile;
+                const int kv_row = (kWindow ? keys.tile(j) : j) * kAttnTile;
                 if (!mbar_wait(&k_empty[ks], kph ^ 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
                 mbar_expect_tx(&k_full[ks], kAttnTileBytes);
-                uint8_t* k = sK + ks * kAttnTileBytes;
-                tma_load_2d(k, &tm_qkv, &k_full[ks], col_k, kv_row);
-                tma_load_2d(k + kAttnSub, &tm_qkv, &k_full[ks], col_k + 64, kv_row);
+                load_tile<kWindow>(sK + ks * kAttnTileBytes, &tm_qkv, &k_full[ks], col_k, b, p.S, kv_row);
                 if (!mbar_wait(&v_empty[slot], ph ^ 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
                 mbar_expect_tx(&v_full[slot], kAttnTileBytes);
-                uint8_t* v = sV + slot * kAttnTileBytes;
-                tma_load_2d(v, &tm_qkv, &v_full[slot], col_v, kv_row);
-                tma_load_2d(v + kAttnSub, &tm_qkv, &v_full[slot], col_v + 64, kv_row);
+                load_tile<kWindow>(sV + slot * kAttnTileBytes, &tm_qkv, &v_full[slot], col_v, b, p.S, kv_row);
                 if (++ks == 3) {
                     ks = 0;
                     kph ^= 1;
@@ -695,8 +768,9 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
         const int grp = (warp - 4) >> 2;       // which 32 of the step's 128 key columns
         const uint32_t lane_bits = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const long long vec = (static_cast<long long>(b) * p.nh + h) * p.S + i * kAttnTile + r;
-        const float lse2 = p.lse[vec] * 1.4426950408889634f;
-        const float dl = p.delta[vec];
+        const bool there = !kWindow || i * kAttnTile + r < p.S;
+        const float lse2 = there ? p.lse[vec] * 1.4426950408889634f : INFINITY;
+        const float dl = there ? p.delta[vec] : 0.f;
         const int kb = grp * 32;   // first of this warp's 32 key columns
         const uint32_t tdPg = tdP + lane_bits + kb;
         bool ok = true;
@@ -710,7 +784,10 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
             tmem_ld_wait();
             tc_fence_before();
             mbar_arrive_warp(&s_empty[buf]);
-            if (j == i) prob_rows<true>(pr, lse2, p.scale_log2, r, kb);
+            const int kt = kWindow ? keys.tile(j) : j;
+            const int last = (i - kt) * kAttnTile + r - kb;
+            if (kWindow ? window_masks(p.win, i, kt) : j == i)
+                prob_rows<true, kWindow>(pr, lse2, p.scale_log2, r, kb, last, last - p.win.window, p.win.sinks - kt * kAttnTile - kb);
             else prob_rows<false>(pr, lse2, p.scale_log2, r, kb);
             if (!mbar_wait_warp(dp_full, j & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
             tc_fence_after();
@@ -734,11 +811,12 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
         }
         bar_sync_compute();
         if (ok) {
-            const long long ld = static_cast<long long>(p.nh + 2 * p.nkv) * kAttnHD;
+            const long long ld = kWindow ? p.ldq : static_cast<long long>(p.nh + 2 * p.nkv) * kAttnHD;
             __nv_bfloat16* dst0 = p.dqkv + (static_cast<long long>(row_base) + i * kAttnTile) * ld + col_q;
             __nv_bfloat16* const dst[2] = {dst0, nullptr};
             const float mul[2] = {p.scale, 0.f};
-            write_staged<false, 2>(stage, dst, mul, ld, threadIdx.x - 128, p.rope ? p.rope + static_cast<long long>(i) * kAttnTile * 64 : nullptr);
+            if constexpr (kWindow) write_staged<false, 2, true>(stage, dst, mul, ld, threadIdx.x - 128, nullptr, p.S - i * kAttnTile);
+            else write_staged<false, 2>(stage, dst, mul, ld, threadIdx.x - 128, p.rope ? p.rope + static_cast<long long>(i) * kAttnTile * 64 : nullptr);
         }
     }
 
@@ -757,6 +835,7 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
 // launches and one: 8 x 384 tokens, 12 / 4 heads (96 and 288 CTAs) 73.9 -> 65.4 us; 7 x 256, 4 / 2 heads 45.3 -> 41.9; 3 x 2432, 32 / 8 heads
 // 854 -> 837; 8192 tokens, 32 / 8 heads 2504 -> 2466. A chain of split heads (AttnBwdParams) waits only for CTAs of lower number, and dQ's CTAs wait
 // for nobody: they leave their SMs to whatever part of the chain is not there yet.
+template <bool kWindow>
 __global__ void __launch_bounds__(kAttnBwdThreads, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do, const AttnBwdParams p,
                 const int dkdv_ctas) {
@@ -768,8 +847,90 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
         return;
     }
     const int cta = static_cast<int>(blockIdx.x);
-    if (cta < dkdv_ctas) attn_dkdv(tm_qkv, tm_do, p, smem, cta);
-    else attn_dq(tm_qkv, tm_do, p, smem, cta - dkdv_ctas);
+    if (cta < dkdv_ctas) attn_dkdv<kWindow>(tm_qkv, tm_do, p, smem, cta);
+    else attn_dq<kWindow>(tm_qkv, tm_do, p, smem, cta - dkdv_ctas);
+}
+
+constexpr int kAttnBwdSmem = 7 * kAttnTileBytes + 2048 + 256;
+template <bool kWindow>
+int configure_bwd(int dev) {
+    static bool configured[64] = {};
+    if (!configured[dev & 63]) {
+        if (cudaFuncSetAttribute(attn_bwd_kernel<kWindow>, cudaFuncAttributeMaxDynamicSharedMemorySize, kAttnBwdSmem) != cudaSuccess) {
+            set_last_error("cudaFuncSetAttribute(attn_bwd) failed");
+            return CAI_K_CUDA;
+        }
+        configured[dev & 63] = true;
+    }
+    return CAI_K_OK;
+}
+
+// ---------------------------------------------------------------------------- the windowed form's parts
+// A key tile's parts added up, in order, to its bf16 rows of dK (times the scale) and dV: those of the window first, head part by head part, then
+// those of the query tiles behind it. Sixteen CTAs a tile, a thread eight columns of one row of one of the two.
+__global__ void __launch_bounds__(256)
+attn_window_join_kernel(const AttnBwdParams p) {
+    grid_dep_begin();
+    const int lin = blockIdx.x >> 4, item = (blockIdx.x & 15) * 256 + threadIdx.x;
+    const int heads_all = p.nkv * p.B, j = lin / heads_all, g = lin % heads_all % p.nkv, b = lin % heads_all / p.nkv;
+    const int nq = (p.S + kAttnTile - 1) / kAttnTile, near_last = window_last_query_tile(p.win, j, nq);
+    const int far = j < p.cut.sink_tiles ? nq - 1 - near_last : 0;      // query tiles behind the window
+    if (p.cut.head_parts == 1 && far <= 0) return;
+    const int which = item >> 11, r = (item >> 4) & 127, c = (item & 15) * 2;
+    if (j * kAttnTile + r >= p.S) return;
+    const uint32_t at0 = which * 65536 + r * 512 + ((c ^ (r & 7)) << 4), at1 = which * 65536 + r * 512 + (((c + 1) ^ (r & 7)) << 4);
+    const char* partial = reinterpret_cast<const char*>(p.partial);
+    const int stride = heads_all * p.cut.head_parts;     // slots of one key tile, of one far part
+    const int mine = (b * p.nkv + g) * p.cut.head_parts;
+    float4 s0 = make_float4(0.f, 0.f, 0.f, 0.f), s1 = s0;
+    auto add = [&](long long slot) {
+        const float4 a = *reinterpret_cast<const float4*>(partial + slot * 131072 + at0), d = *reinterpret_cast<const float4*>(partial + slot * 131072 + at1);
+        s0.x += a.x; s0.y += a.y; s0.z += a.z; s0.w += a.w;
+        s1.x += d.x; s1.y += d.y; s1.z += d.z; s1.w += d.w;
+    };
+    for (int k = 0; k < p.cut.head_parts; ++k) add(static_cast<long long>(j) * stride + mine + k);
+    const int parts = far > 0 ? (far + p.cut.far_tiles - 1) / p.cut.far_tiles : 0;
+    const long long far0 = p.cut.near_slots + static_cast<long long>(j) * p.cut.far_parts * stride + mine;
+#pragma unroll 4
+    for (int f = 0; f < parts; ++f)
+        for (int k = 0; k < p.cut.head_parts; ++k) add(far0 + static_cast<long long>(f) * stride + k);
+    const float mul = which ? 1.f : p.scale;
+    const int col = (which ? p.nh + p.nkv + g : p.nh + g) * kAttnHD + c * 4;
+    *reinterpret_cast<uint4*>(p.dqkv + (static_cast<long long>(b) * p.S + j * kAttnTile + r) * p.ldq + col) =
+        make_uint4(pack_bf16(s0.x * mul, s0.y * mul), pack_bf16(s0.z * mul, s0.w * mul), pack_bf16(s1.x * mul, s1.y * mul), pack_bf16(s1.z * mul, s1.w * mul));
+}
+
+// Whole numbers only, so that host and device agree on every size. Cutting is worth it where one CTA's steps would outlast everybody's share of all steps:
+// dK / dV of a step cost about 5 / 4 of dQ's.
+AttnWindowParts window_parts(const AttnWindow& w, int B, int S, int nh, int nkv, int sms) {
+    AttnWindowParts c = {};
+    const int nq = (S + kAttnTile - 1) / kAttnTile, rep = nh / nkv;
+    const long long groups = static_cast<long long>(B) * nkv;
+    const int near_most = window_last_query_tile(w, 0, nq) + 1, far_most = nq - near_most;
+    const int sink_all = (w.sinks + kAttnTile - 1) / kAttnTile;
+    while (c.sink_tiles < sink_all && window_last_query_tile(w, c.sink_tiles, nq) + 1 < nq) ++c.sink_tiles;
+    long long steps = 0;     // of one head, in quarters of a dQ step
+    for (int j = 0; j < nq; ++j) steps += 9ll * (j < c.sink_tiles ? nq - j : window_last_query_tile(w, j, nq) - j + 1);
+    const long long share = steps * B * nh / sms;
+    c.head_parts = 1;
+    const long long join = 12;   // what the second kernel costs beyond its launch behind sink tiles, in the same unit
+    for (int k = 2; k <= rep; ++k)
+        if (rep % k == 0) {
+            const long long now = 5ll * near_most * (rep / c.head_parts), then = 5ll * near_most * (rep / k);
+            if ((now > share ? now : share) > (then > share ? then : share) + (c.head_parts == 1 && !c.sink_tiles ? join : 0)) c.head_parts = k;
+        }
+    const long long heads_all = groups * c.head_parts;
+    if (c.sink_tiles) {
+        // no shorter than a window, and no more of them than about one a SM
+        long long tiles = (far_most * c.sink_tiles * heads_all + sms - 1) / sms;
+        tiles = tiles > near_most ? tiles : near_most;
+        c.far_tiles = static_cast<int>(tiles < far_most ? tiles : far_most);
+        c.far_parts = (far_most + c.far_tiles - 1) / c.far_tiles;
+    }
+    c.near_ctas = static_cast<int>(nq * heads_all);
+    c.far_ctas = static_cast<int>(c.sink_tiles * heads_all * c.far_parts);
+    c.near_slots = static_cast<int>(c.head_parts > 1 ? c.near_ctas : c.sink_tiles * heads_all);
+    return c;
 }
 
 }  // namespace cai
@@ -803,17 +964,9 @@ CAI_API int cai_flash_attn_bwd_rope(const void* qkv, const void* out, const void
     CUtensorMap tm_qkv, tm_do;
     if (!encode_tmap_2d(&tm_qkv, qkv, static_cast<uint64_t>(B) * S, ld, ld, 64, kAttnTile, 2)) return CAI_K_BAD_ARG;
     if (!encode_tmap_2d(&tm_do, dout, static_cast<uint64_t>(B) * S, ldo, ldo, 64, kAttnTile, 2)) return CAI_K_BAD_ARG;
-    constexpr int smem_bytes = 7 * kAttnTileBytes + 2048 + 256;
-    static bool configured[64] = {};
     const int dev = current_device();
-    if (!configured[dev & 63]) {
-        if (cudaFuncSetAttribute(attn_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess) {
-            set_last_error("cudaFuncSetAttribute(attn_bwd) failed");
-            return CAI_K_CUDA;
-        }
-        configured[dev & 63] = true;
-    }
-    AttnBwdParams p;
+    if (configure_bwd<false>(dev)) return CAI_K_CUDA;
+    AttnBwdParams p = {};
     p.B = B; p.S = S; p.nh = nh; p.nkv = nkv;
     p.scale = scale;
     p.scale_log2 = scale * 1.4426950408889634f;
@@ -855,11 +1008,90 @@ CAI_API int cai_flash_attn_bwd_rope(const void* qkv, const void* out, const void
     const long long kv_ctas = (parts & 2) ? static_cast<long long>(nq) * (p.split_heads ? nh : nkv) * B : 0;
     const long long q_ctas = (parts & 4) ? static_cast<long long>(nq) * nh * B : 0;
     if (kv_ctas + q_ctas)
-        launch_early(attn_bwd_kernel, static_cast<unsigned>(kv_ctas + q_ctas), kAttnBwdThreads, smem_bytes, st, tm_qkv, tm_do, p,
+        launch_early(attn_bwd_kernel<false>, static_cast<unsigned>(kv_ctas + q_ctas), kAttnBwdThreads, kAttnBwdSmem, st, tm_qkv, tm_do, p,
                      static_cast<int>(kv_ctas));
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
         set_last_error("attn_bwd launch failed: %s", cudaGetErrorString(e));
+        return CAI_K_CUDA;
+    }
+    return CAI_K_OK;
+}
+
+CAI_API int cai_flash_attn_window_walk(int B, int S, int nh, int nkv, int window, int sinks, int sms, int* parts, int capacity) {
+    const AttnWindow w = {window < S ? window : S, sinks < S ? sinks : S};
+    const AttnWindowParts c = window_parts(w, B, S, nh, nkv, sms);
+    const int n = c.near_ctas + c.far_ctas;
+    for (int lin = 0; lin < n && lin < capacity; ++lin) {
+        const WindowPart t(w, c, B, S, nh, nkv, lin);
+        const int v[8] = {t.j, t.b, t.g, t.h_first, t.heads, t.q_first, t.q_tiles, t.slot};
+        for (int k = 0; k < 8; ++k) parts[lin * 8 + k] = v[k];
+    }
+    return n;
+}
+CAI_API int cai_flash_attn_window_keys(int S, int window, int sinks, int i, int* tiles, int capacity) {
+    const WindowKeys keys({window < S ? window : S, sinks < S ? sinks : S}, i);
+    for (int k = 0; k < keys.n && k < capacity; ++k) tiles[k] = keys.tile(k);
+    return keys.n;
+}
+
+CAI_API long long cai_flash_attn_window_bwd_scratch(int B, int S, int nh, int nkv, int window, int sinks) {
+    if (B <= 0 || S <= 0 || nkv <= 0 || nh < nkv || nh % nkv || window < 1 || sinks < 0) return 0;
+    const int sms = sm_count(current_device());
+    const AttnWindowParts c = window_parts({window < S ? window : S, sinks < S ? sinks : S}, B, S, nh, nkv, sms > 0 ? sms : 148);
+    return (static_cast<long long>(c.near_slots) + c.far_ctas) * 131072;
+}
+
+CAI_API int cai_flash_attn_window_bwd(const void* qkv, long long ld, const void* out, const void* dout, const float* lse, float* delta, void* dqkv,
+                                      long long ldq, void* scratch, int B, int S, int nh, int nkv, int hd, float scale, int window, int sinks,
+                                      void* stream) {
+    if (!window_call_ok("flash_attn_window_bwd", qkv, ld, out, B, S, nh, nkv, hd, window, sinks) ||
+        !window_call_ok("flash_attn_window_bwd (gradient)", dqkv, ldq, dout, B, S, nh, nkv, hd, window, sinks))
+        return CAI_K_BAD_ARG;
+    if (B == 0 || S == 0) return CAI_K_OK;
+    if (reinterpret_cast<uintptr_t>(scratch) & 15) {
+        set_last_error("flash_attn_window_bwd: the scratch has to start on 16 bytes");
+        return CAI_K_BAD_ARG;
+    }
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const long long ldo = static_cast<long long>(nh) * hd;
+    CUtensorMap tm_qkv, tm_do;
+    if (!encode_tmap_3d(&tm_qkv, qkv, static_cast<uint64_t>(nh + 2 * nkv) * hd, S, B, ld, static_cast<uint64_t>(ld) * S, 64, kAttnTile, 2) ||
+        !encode_tmap_3d(&tm_do, dout, ldo, S, B, ldo, static_cast<uint64_t>(ldo) * S, 64, kAttnTile, 2))
+        return CAI_K_BAD_ARG;
+    const int dev = current_device();
+    if (configure_bwd<true>(dev)) return CAI_K_CUDA;
+    AttnBwdParams p = {};
+    p.B = B; p.S = S; p.nh = nh; p.nkv = nkv;
+    p.scale = scale;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    p.lse = lse;
+    p.delta = delta;
+    p.dqkv = static_cast<__nv_bfloat16*>(dqkv);
+    p.ldq = ldq;
+    p.status = status_words(dev);
+    p.win = {window < S ? window : S, sinks < S ? sinks : S};
+    p.cut = window_parts(p.win, B, S, nh, nkv, sm_count(dev));
+    p.partial = static_cast<float*>(scratch);
+    if (!scratch && p.cut.near_slots + p.cut.far_ctas > 0) {
+        set_last_error("flash_attn_window_bwd: needs the scratch that cai_flash_attn_window_bwd_scratch says");
+        return CAI_K_BAD_ARG;
+    }
+    const long long rows = static_cast<long long>(B) * S * nh;
+    constexpr unsigned per_cta = 16u * kDeltaUnroll;
+    cudaError_t e = launch_early(attn_delta_kernel, static_cast<unsigned>((rows + per_cta - 1) / per_cta), 256, 0, st,
+                                 static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(dout), delta, static_cast<unsigned>(rows),
+                                 static_cast<unsigned>(S), static_cast<unsigned>(nh), true, static_cast<unsigned int*>(nullptr), 0u);
+    const int kv_ctas = p.cut.near_ctas + p.cut.far_ctas;
+    const long long q_ctas = static_cast<long long>((S + kAttnTile - 1) / kAttnTile) * nh * B;
+    if (e == cudaSuccess)
+        e = launch_early(attn_bwd_kernel<true>, static_cast<unsigned>(kv_ctas + q_ctas), kAttnBwdThreads, kAttnBwdSmem, st, tm_qkv, tm_do, p, kv_ctas);
+    if (e == cudaSuccess && p.cut.near_slots + p.cut.far_ctas > 0) {
+        const long long tiles = p.cut.head_parts > 1 ? (S + kAttnTile - 1) / kAttnTile : p.cut.sink_tiles;
+        e = launch_early(attn_window_join_kernel, static_cast<unsigned>(tiles * nkv * B * 16), 256, 0, st, p);
+    }
+    if (e != cudaSuccess) {
+        set_last_error("flash_attn_window_bwd launch failed: %s", cudaGetErrorString(e));
         return CAI_K_CUDA;
     }
     return CAI_K_OK;

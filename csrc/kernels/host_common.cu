@@ -122,6 +122,28 @@ bool encode_tmap_3d(CUtensorMap* out, const void* base, uint64_t cols, uint64_t 
     return true;
 }
 
+bool window_call_ok(const char* name, const void* qkv, long long ld, const void* out, int B, int S, int nh, int nkv, int hd, int window, int sinks) {
+    if (hd != 128 || nkv <= 0 || nh <= 0 || nh % nkv || B < 0 || S < 0) {
+        set_last_error("%s: needs head_dim 128 and heads %% kv_heads == 0 (hd=%d, %d heads, %d kv heads, B=%d, S=%d)", name, hd, nh, nkv, B, S);
+        return false;
+    }
+    if (window < 1 || sinks < 0) {
+        set_last_error("%s: a token sees itself: the window has to be 1 or more, the sinks 0 or more (%d, %d)", name, window, sinks);
+        return false;
+    }
+    // rows and columns are counted in 32 bits, query tiles of all heads are the grid's (y and z up to 65535)
+    const long long rows = static_cast<long long>(B) * S, cols = (static_cast<long long>(nh) + 2ll * nkv) * hd;
+    if (rows * nh > 0x3fffffffll || S > 0x7fffffff - 256 || cols > 0x7fffffffll || B > 65535 || nh > 65535) {
+        set_last_error("%s: too many rows or heads (B=%d, S=%d, %d heads)", name, B, S, nh);
+        return false;
+    }
+    if (ld < cols || (ld & 7) || (reinterpret_cast<uintptr_t>(qkv) & 15) || (reinterpret_cast<uintptr_t>(out) & 15)) {
+        set_last_error("%s: rows have to hold all heads and start on 16 bytes (pitch %lld, %lld columns)", name, ld, cols);
+        return false;
+    }
+    return true;
+}
+
 }  // namespace cai
 
 // ---- exported status API -------------------------------------------------------------

@@ -34,7 +34,7 @@ bool take(PyObject* o, T& out) {
 }
 
 template <auto kFunction> struct Call;
-template <typename... Args, int (*kFunction)(Args...)> struct Call<kFunction> {
+template <typename R, typename... Args, R (*kFunction)(Args...)> struct Call<kFunction> {
     static PyObject* run(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (n != static_cast<Py_ssize_t>(sizeof...(Args))) {
             PyErr_Format(PyExc_TypeError, "%zu arguments are wanted, %zd given", sizeof...(Args), n);
@@ -46,11 +46,11 @@ template <typename... Args, int (*kFunction)(Args...)> struct Call<kFunction> {
     static PyObject* go(PyObject* const* args, std::index_sequence<I...>) {
         std::tuple<Args...> v;
         if (!(take(args[I], std::get<I>(v)) && ...)) return nullptr;
-        int rc;
+        R rc;
         Py_BEGIN_ALLOW_THREADS
         rc = kFunction(std::get<I>(v)...);
         Py_END_ALLOW_THREADS
-        return PyLong_FromLong(rc);
+        return PyLong_FromLongLong(rc);
     }
 };
 
@@ -63,6 +63,8 @@ PyMethodDef functions[] = {
     CAI_CALL(cai_rope_table), CAI_CALL(cai_rope_apply), CAI_CALL(cai_swiglu_fwd), CAI_CALL(cai_swiglu_bwd),
     CAI_CALL(cai_embed_fwd), CAI_CALL(cai_embed_bwd), CAI_CALL(cai_cross_entropy), CAI_CALL(cai_adamw),
     CAI_CALL(cai_flash_attn_fwd_variant), CAI_CALL(cai_flash_attn_bwd_parts),
+    CAI_CALL(cai_add_rmsnorm_quant), CAI_CALL(cai_rope_apply_axes),
+    CAI_CALL(cai_flash_attn_window_fwd), CAI_CALL(cai_flash_attn_window_bwd_scratch), CAI_CALL(cai_flash_attn_window_bwd),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, functions, nullptr, nullptr, nullptr, nullptr};

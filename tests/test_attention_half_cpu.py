@@ -1,0 +1,200 @@
+"""Windowed attention, rotary positions of several axes and the e4m3 norm, as far as no GPU is needed: which tiles the CTAs of windowed attention take, and what
+the calls refuse."""
+import ctypes
+
+import pytest
+import torch
+
+T = 128
+
+
+def _seen(i, j, window, sinks):
+    return j <= i and (j > i - window or j < sinks)
+
+
+def _tile_pairs(S, window, sinks):
+    """(query tile, key tile) of every pair of tiles in which some query sees some key."""
+    n = (S + T - 1) // T
+    found = set()
+    for i in range(n):
+        for j in range(i + 1):
+            q_last, k_first, k_last = min(S, (i + 1) * T) - 1, j * T, min(S, (j + 1) * T) - 1
+            # the nearest pair decides for the window, the first key for the sinks
+            nearest = max(i * T, k_first) - min(k_last, i * T) if i > j else 0
+            if nearest < window or k_first < sinks:
+                assert k_first <= q_last
+                found.add((i, j))
+    return found
+
+
+SHAPES = [(1, 1, 1, 1, 1, 0), (2, 128, 2, 1, 64, 4), (3, 129, 4, 2, 1, 0), (1, 1000, 9, 3, 200, 0), (1, 333, 8, 1, 512, 1), (4, 4096, 16, 8, 1024, 4),
+          (1, 8192, 4, 1, 128, 130), (1, 8192, 8, 8, 2, 512), (2, 2000, 6, 2, 129, 127), (1, 5000, 8, 1, 257, 5000), (7, 640, 3, 3, 128, 128),
+          (1, 16384, 2, 1, 300, 1), (1, 3000, 16, 2, 127, 300)]
+
+
+@pytest.mark.parametrize("B,S,nh,nkv,window,sinks", SHAPES)
+def test_forward_takes_every_key_tile_once(B, S, nh, nkv, window, sinks):
+    from cai_b200.ops import lib
+    want = _tile_pairs(S, window, sinks)
+    got = []
+    for i in range((S + T - 1) // T):
+        tiles = (ctypes.c_int * 4096)()
+        n = lib().cai_flash_attn_window_keys(S, window, sinks, i, tiles, 4096)
+        assert 0 < n <= 4096 and tiles[0] == i, "the diagonal tile comes first"
+        got += [(i, tiles[k]) for k in range(n)]
+    assert len(got) == len(set(got))
+    assert set(got) == want
+
+
+@pytest.mark.parametrize("sms", [148, 8, 1])
+@pytest.mark.parametrize("B,S,nh,nkv,window,sinks", SHAPES)
+def test_backward_parts_cover_every_sum_once(B, S, nh, nkv, window, sinks, sms):
+    """Every (batch, query head, query tile, key tile) lies in one CTA's part; parts of one key tile have scratch of their own, or the tile has one part."""
+    from cai_b200.ops import lib
+    n = lib().cai_flash_attn_window_walk(B, S, nh, nkv, window, sinks, sms, None, 0)
+    parts = (ctypes.c_int * (8 * n))()
+    assert lib().cai_flash_attn_window_walk(B, S, nh, nkv, window, sinks, sms, parts, n) == n
+    seen, slots, of_tile = set(), set(), {}
+    for c in range(n):
+        j, b, g, h0, heads, q0, tiles, slot = parts[8 * c:8 * c + 8]
+        assert 0 <= b < B and 0 <= g < nkv and heads >= 1 and g * (nh // nkv) <= h0 and h0 + heads <= (g + 1) * (nh // nkv)
+        if tiles <= 0:
+            continue
+        assert 0 <= j <= q0 and (q0 + tiles - 1) * T < S
+        of_tile.setdefault((b, g, j), []).append(slot)
+        assert slot < 0 or slot not in slots
+        slots.add(slot)
+        for h in range(h0, h0 + heads):
+            for i in range(q0, q0 + tiles):
+                assert (b, h, i, j) not in seen
+                seen.add((b, h, i, j))
+    want = _tile_pairs(S, window, sinks)
+    assert seen == {(b, h, i, j) for b in range(B) for h in range(nh) for i, j in want}
+    assert len(of_tile) == B * nkv * ((S + T - 1) // T), "every key tile's rows are written"
+    for s in of_tile.values():
+        assert len(s) == 1 and s[0] == -1 or min(s) >= 0
+    if sms == 148:
+        most = lib().cai_flash_attn_window_bwd_scratch(B, S, nh, nkv, window, sinks)
+        assert max(slots) * 131072 + 131072 <= most or max(slots) < 0
+
+
+def test_parts_of_sink_tiles_are_no_longer_than_a_share():
+    """One kv head of a very long sequence: the first tile's 256 query tiles are cut into parts, the scratch stays that of about one part a SM."""
+    from cai_b200.ops import lib
+    B, S, nh, nkv, window, sinks = 1, 32768, 4, 1, 2048, 130
+    n = lib().cai_flash_attn_window_walk(B, S, nh, nkv, window, sinks, 148, None, 0)
+    parts = (ctypes.c_int * (8 * n))()
+    lib().cai_flash_attn_window_walk(B, S, nh, nkv, window, sinks, 148, parts, n)
+    steps = [parts[8 * c + 4] * max(0, parts[8 * c + 6]) for c in range(n)]
+    assert max(steps) <= 2 * 4 * (2048 // T + 1)
+    assert lib().cai_flash_attn_window_bwd_scratch(B, S, nh, nkv, window, sinks) <= 2 * 148 * 2 * 131072
+
+
+# ---------------------------------------------------------------------------- refusals
+P = 1 << 20      # an address that no refused call looks at
+
+
+def _window(name, **change):
+    a = dict(qkv=P, ld=512, out=P, lse=P, dout=P, delta=P, dqkv=P, ldq=512, scratch=P, B=1, S=256, nh=2, nkv=1, hd=128, scale=0.1, window=64, sinks=4, stream=0)
+    a.update(change)
+    if name == "fwd":
+        order = ("qkv", "ld", "out", "lse", "B", "S", "nh", "nkv", "hd", "scale", "window", "sinks", "stream")
+    else:
+        order = ("qkv", "ld", "out", "dout", "lse", "delta", "dqkv", "ldq", "scratch", "B", "S", "nh", "nkv", "hd", "scale", "window", "sinks", "stream")
+    return [a[k] for k in order]
+
+
+BAD_WINDOW = [dict(hd=64), dict(nh=3, nkv=2, ld=1024, ldq=1024), dict(nkv=0), dict(nh=0), dict(window=0), dict(window=-5), dict(sinks=-1), dict(ld=504, ldq=504),
+              dict(ld=516, ldq=516), dict(qkv=P + 8), dict(out=P + 8), dict(B=-1), dict(S=-1), dict(B=70000), dict(B=60000, S=60000)]
+
+
+@pytest.mark.parametrize("change", BAD_WINDOW, ids=str)
+@pytest.mark.parametrize("name", ["fwd", "bwd"])
+def test_window_launchers_refuse(name, change):
+    from cai_b200.ops import KernelError, calls, check
+    f = getattr(calls(), f"cai_flash_attn_window_{name}")
+    with pytest.raises(KernelError, match="flash_attn_window"):
+        check(f(*_window(name, **change)), "flash_attn_window")
+
+
+@pytest.mark.parametrize("change", [dict(dout=P + 2), dict(dqkv=P + 4), dict(ldq=500), dict(scratch=P + 4)], ids=str)
+def test_window_bwd_launcher_refuses(change):
+    from cai_b200.ops import KernelError, calls, check
+    with pytest.raises(KernelError, match="flash_attn_window_bwd"):
+        check(calls().cai_flash_attn_window_bwd(*_window("bwd", **change)), "flash_attn_window")
+
+
+@pytest.mark.parametrize("name", ["fwd", "bwd"])
+@pytest.mark.parametrize("change", [dict(B=0), dict(S=0)], ids=str)
+def test_window_launchers_do_nothing_for_no_rows(name, change):
+    from cai_b200.ops import calls
+    assert getattr(calls(), f"cai_flash_attn_window_{name}")(*_window(name, **change)) == 0
+
+
+def test_window_calls_refuse_tensors_that_do_not_fit():
+    from cai_b200 import ops
+    B, S, nh, nkv = 2, 10, 2, 1
+    qkv = torch.zeros(B * S, 4 * 128, dtype=torch.bfloat16)
+    out, lse = torch.zeros(B * S, 256, dtype=torch.bfloat16), torch.zeros(B, nh, S)
+    for bad in (qkv.float(), qkv[1:], qkv[:, 1:], qkv.t(), qkv.view(-1).as_strided((B * S, 512), (256, 1))):
+        with pytest.raises(ops.KernelError, match="flash_attn_window_fwd"):
+            ops.flash_attn_window_fwd(bad, B, S, nh, nkv, 128, 4)
+        with pytest.raises(ops.KernelError, match="flash_attn_window_bwd"):
+            ops.flash_attn_window_bwd(bad, out, out, lse, B, S, nh, nkv, 128, 4)
+    for o, d, l in ((out.float(), out, lse), (out, out[:, :128], lse), (out, out, lse.double()), (out, out, lse[:, :1]), (out, out.t().contiguous().t(), lse)):
+        with pytest.raises(ops.KernelError, match="flash_attn_window_bwd"):
+            ops.flash_attn_window_bwd(qkv, o, d, l, B, S, nh, nkv, 128, 4)
+
+
+def _rope(**change):
+    a = dict(qkv=P, freqs=P, pos=P, ldp=10, T=10, nh=2, nkv=1, hd=128, ld=512, axes=3, n0=16, n1=24, n2=24, n3=0, interleaved=0, inverse=0, stream=0)
+    a.update(change)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change", [dict(hd=120), dict(hd=272), dict(hd=0), dict(axes=0), dict(axes=5), dict(n0=15), dict(n3=1, n0=15), dict(n0=-8, n1=48), dict(ld=380),
+                                    dict(ld=376), dict(qkv=P + 2), dict(ldp=9), dict(T=-1), dict(interleaved=1)], ids=str)
+def test_rope_launcher_refuses(change):
+    from cai_b200.ops import KernelError, calls, check
+    with pytest.raises(KernelError, match="rope_apply_axes"):
+        check(calls().cai_rope_apply_axes(*_rope(**change)), "rope")
+
+
+def test_rope_call_refuses_tensors_that_do_not_fit():
+    from cai_b200 import ops
+    qkv, freqs, pos = torch.zeros(10, 512, dtype=torch.bfloat16), torch.zeros(64, dtype=torch.float64), torch.zeros(3, 10, dtype=torch.int32)
+    good = dict(qkv=qkv, freqs=freqs, pos=pos, nh=2, nkv=1, hd=128, sections=(16, 24, 24))
+    for change in (dict(qkv=qkv.float()), dict(qkv=qkv[:, :256]), dict(qkv=qkv.t()), dict(qkv=qkv[:, ::2]), dict(freqs=freqs.float()), dict(freqs=freqs[:32]), dict(pos=pos.long()),
+                   dict(pos=pos[:2]), dict(pos=pos[:, :9]), dict(pos=torch.zeros(10, 3, dtype=torch.int32).t()), dict(sections=()), dict(sections=(16, 16, 16, 8, 8))):
+        with pytest.raises(ops.KernelError, match="rope_apply_axes_"):
+            ops.rope_apply_axes_(**{**good, **change})
+
+
+def _norm(**change):
+    a = dict(x=P, ldx=256, residual=P, ldr=256, g=P, h=P, y=P, q=P, scale=P, rstd=P, rows=4, H=256, eps=1e-6, stream=0)
+    a.update(change)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("change", [dict(H=192), dict(H=16512), dict(H=0), dict(rows=-1), dict(ldx=252), dict(ldr=260), dict(x=P + 2), dict(residual=P + 8), dict(g=P + 8),
+                                    dict(h=P + 8), dict(y=P + 4), dict(q=P + 1)], ids=str)
+def test_norm_launcher_refuses(change):
+    from cai_b200.ops import KernelError, calls, check
+    with pytest.raises(KernelError, match="add_rmsnorm_quant"):
+        check(calls().cai_add_rmsnorm_quant(*_norm(**change)), "norm")
+
+
+def test_norm_call_refuses_tensors_that_do_not_fit():
+    from cai_b200 import ops
+    x, g = torch.zeros(4, 256, dtype=torch.bfloat16), torch.zeros(256, dtype=torch.bfloat16)
+    for a in ((x.float(), None, g), (x, None, g.float()), (x, None, g[:128]), (x, x[:2], g), (x, x.float(), g), (x[:, ::2], None, g[:128]), (x.view(2, 2, 256), None, g),
+              (x, torch.zeros(256, 4, dtype=torch.bfloat16).t(), g)):
+        with pytest.raises(ops.KernelError, match="add_rmsnorm_quant"):
+            ops.add_rmsnorm_quant(*a)
+
+
+def test_frequencies():
+    from cai_b200 import ops
+    f = ops.rope_freqs(128, 500000.0, device="cpu")
+    assert f.dtype == torch.float64 and f.shape == (64,) and f[0] == 1.0
+    assert abs(f[32].item() - 500000.0 ** -0.5) < 1e-15
