@@ -22,8 +22,7 @@ __device__ __forceinline__ float fast_exp2(float x) {
 struct AttnWindow {
     int window, sinks;
 };
-// The key tiles of query tile i: from the diagonal down to the one that holds the first query's first key, then the sinks' tiles below it. The diagonal
-// comes first because every row sees a key there: the running maximum is finite from the first step on, whatever the later tiles hide.
+// The key tiles of query tile i, in ascending order: the sinks' tiles, then those from the one that holds the first query's first key up to the diagonal.
 struct WindowKeys {
     int diag, near, n;
     __host__ __device__ WindowKeys(const AttnWindow& w, int i) {
@@ -32,7 +31,7 @@ struct WindowKeys {
         near = i - lo + 1;
         n = near + (sink_tiles < lo ? sink_tiles : lo);
     }
-    __host__ __device__ int tile(int j) const { return j < near ? diag - j : j - near; }
+    __host__ __device__ int tile(int j) const { return j < n - near ? j : diag - (n - 1 - j); }
 };
 // The query tiles that key tile j is seen by through the window: j .. last.
 __host__ __device__ inline int window_last_query_tile(const AttnWindow& w, int j, int tiles) {

@@ -1045,8 +1045,8 @@ CAI_API long long cai_flash_attn_window_bwd_scratch(int B, int S, int nh, int nk
 CAI_API int cai_flash_attn_window_bwd(const void* qkv, long long ld, const void* out, const void* dout, const float* lse, float* delta, void* dqkv,
                                       long long ldq, void* scratch, int B, int S, int nh, int nkv, int hd, float scale, int window, int sinks,
                                       void* stream) {
-    if (!window_call_ok("flash_attn_window_bwd", qkv, ld, out, B, S, nh, nkv, hd, window, sinks) ||
-        !window_call_ok("flash_attn_window_bwd (gradient)", dqkv, ldq, dout, B, S, nh, nkv, hd, window, sinks))
+    if (!window_call_ok("flash_attn_window_bwd", qkv, ld, out, B, S, nh, nkv, hd, scale, window, sinks) ||
+        !window_call_ok("flash_attn_window_bwd (gradient)", dqkv, ldq, dout, B, S, nh, nkv, hd, scale, window, sinks))
         return CAI_K_BAD_ARG;
     if (B == 0 || S == 0) return CAI_K_OK;
     if (reinterpret_cast<uintptr_t>(scratch) & 15) {

@@ -122,9 +122,13 @@ bool encode_tmap_3d(CUtensorMap* out, const void* base, uint64_t cols, uint64_t 
     return true;
 }
 
-bool window_call_ok(const char* name, const void* qkv, long long ld, const void* out, int B, int S, int nh, int nkv, int hd, int window, int sinks) {
+bool window_call_ok(const char* name, const void* qkv, long long ld, const void* out, int B, int S, int nh, int nkv, int hd, float scale, int window, int sinks) {
     if (hd != 128 || nkv <= 0 || nh <= 0 || nh % nkv || B < 0 || S < 0) {
         set_last_error("%s: needs head_dim 128 and heads %% kv_heads == 0 (hd=%d, %d heads, %d kv heads, B=%d, S=%d)", name, hd, nh, nkv, B, S);
+        return false;
+    }
+    if (!(scale > 0.f) || scale > 3e38f) {
+        set_last_error("%s: the scale has to be positive and finite (%g)", name, scale);   // hidden scores are -inf times it
         return false;
     }
     if (window < 1 || sinks < 0) {

@@ -58,7 +58,7 @@ inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, dim3 block
 }
 
 // The arguments that both directions of windowed attention have in common; says what is wrong with them.
-bool window_call_ok(const char* name, const void* qkv, long long ld, const void* out, int B, int S, int nh, int nkv, int hd, int window, int sinks);
+bool window_call_ok(const char* name, const void* qkv, long long ld, const void* out, int B, int S, int nh, int nkv, int hd, float scale, int window, int sinks);
 
 const char* last_error();
 void set_last_error(const char* fmt, ...);

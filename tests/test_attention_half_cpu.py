@@ -40,7 +40,7 @@ def test_forward_takes_every_key_tile_once(B, S, nh, nkv, window, sinks):
     for i in range((S + T - 1) // T):
         tiles = (ctypes.c_int * 4096)()
         n = lib().cai_flash_attn_window_keys(S, window, sinks, i, tiles, 4096)
-        assert 0 < n <= 4096 and tiles[0] == i, "the diagonal tile comes first"
+        assert 0 < n <= 4096 and list(tiles[:n]) == sorted(tiles[:n]) and tiles[n - 1] == i, "in order, the diagonal last"
         got += [(i, tiles[k]) for k in range(n)]
     assert len(got) == len(set(got))
     assert set(got) == want
@@ -105,7 +105,7 @@ def _window(name, **change):
 
 
 BAD_WINDOW = [dict(hd=64), dict(nh=3, nkv=2, ld=1024, ldq=1024), dict(nkv=0), dict(nh=0), dict(window=0), dict(window=-5), dict(sinks=-1), dict(ld=504, ldq=504),
-              dict(ld=516, ldq=516), dict(qkv=P + 8), dict(out=P + 8), dict(B=-1), dict(S=-1), dict(B=70000), dict(B=60000, S=60000)]
+              dict(ld=516, ldq=516), dict(qkv=P + 8), dict(out=P + 8), dict(scale=0.0), dict(scale=-0.1), dict(scale=float('inf')), dict(scale=float('nan')), dict(B=-1), dict(S=-1), dict(B=70000), dict(B=60000, S=60000)]
 
 
 @pytest.mark.parametrize("change", BAD_WINDOW, ids=str)
