@@ -24,8 +24,36 @@ struct NormQuantParams {
     float eps;
 };
 
+// Two fp32 numbers in one register pair; an instruction of the two takes one issue slot.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 floats_of(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t bf16x2_pair(uint32_t v) { return pair_of(bf16_lo(v), bf16_hi(v)); }
+
+// The scale of a block whose largest magnitude is `amax`. Where 1 / scale would leave fp32's range the block is near enough to zero for a scale that does not.
+__device__ __forceinline__ float block_scale(float amax) { return amax > 0.f ? fmaxf(amax, 0x1p-100f) / 448.f : 1.f; }
+
 // A row is shared by p.warps warps, each lane holding kChunks times eight of its columns in registers, 256 columns of a warp apart: sixteen lanes hold one
-// block of the quantiser. A CTA takes blockDim / (32 * p.warps) rows.
+// block of the quantiser. A CTA takes blockDim / (32 * p.warps) rows. With the residual and y this is bound by its 9 bytes an element, without them, 3 bytes, by
+// its instructions: hence the arithmetic on pairs, and (kChunks = 4) the four blocks' maxima reduced together: a lane that gives two of its
+// four away at the first step and one at the second is left with one, whose scale and reciprocal it computes for the sixteen.
 template <int kChunks>
 __global__ void __launch_bounds__(256)
 add_rmsnorm_quant_kernel(const NormQuantParams p) {
@@ -36,13 +64,17 @@ add_rmsnorm_quant_kernel(const NormQuantParams p) {
     const long long row = static_cast<long long>(blockIdx.x) * groups + grp;
     const bool live = row < p.rows;
     const int col0 = sub * kChunks * 256 + lane * 8;
-    uint4 v[kChunks];
-    float ss = 0.f;
+    uint4 v[kChunks], g[kChunks];
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
         v[c] = make_uint4(0, 0, 0, 0);
         const int col = col0 + c * 256;
         if (live && col < p.H) v[c] = *reinterpret_cast<const uint4*>(p.x + row * p.ldx + col);
+    }
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int col = col0 + c * 256;
+        g[c] = col < p.H ? *reinterpret_cast<const uint4*>(p.g + col) : make_uint4(0, 0, 0, 0);
     }
     if (p.residual) {
         uint4 r[kChunks];
@@ -62,16 +94,20 @@ add_rmsnorm_quant_kernel(const NormQuantParams p) {
             v[c] = pack8(a);
         }
     }
+    uint64_t ss2 = 0;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
         const int col = col0 + c * 256;
         if (p.h && live && col < p.H) *reinterpret_cast<uint4*>(p.h + row * p.H + col) = v[c];
-        float f[8];
-        unpack8(v[c], f);
+        const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+        for (int k = 0; k < 4; ++k) {
+            const uint64_t f = bf16x2_pair(w[k]);
+            ss2 = fma2(f, f, ss2);
+        }
     }
-    ss = warp_sum(ss);
+    const float2 s01 = floats_of(ss2);
+    float ss = warp_sum(s01.x + s01.y);
     if (p.warps > 1) {
         if (lane == 0) part[warp] = ss;
         __syncthreads();
@@ -80,31 +116,60 @@ add_rmsnorm_quant_kernel(const NormQuantParams p) {
     }
     const float rr = 1.f / sqrtf(ss / p.H + p.eps);
     if (live && sub == 0 && lane == 0) p.rstd[row] = rr;
+    const uint64_t rr2 = pair_of(rr, rr);
+    uint64_t y[kChunks][4];
+    float amax[kChunks], inv[kChunks];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w}, gw[4] = {g[c].x, g[c].y, g[c].z, g[c].w};
+        amax[c] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            y[c][k] = mul2(mul2(bf16x2_pair(w[k]), rr2), bf16x2_pair(gw[k]));
+            const float2 f = floats_of(y[c][k]);
+            amax[c] = fmaxf(amax[c], fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+    }
+    auto put_scale = [&](int c, float s) {
+        const int col = sub * kChunks * 256 + c * 256 + (lane >> 4) * 128;
+        if (live && col < p.H) p.scale[row * (p.H >> 7) + (col >> 7)] = s;
+    };
+    if constexpr (kChunks == 4) {
+        // lane bit 3 decides which two of the four a lane keeps, bit 2 which one of them
+        const bool b3 = lane & 8, b2 = lane & 4;
+        const float k0 = fmaxf(b3 ? amax[2] : amax[0], __shfl_xor_sync(0xffffffffu, b3 ? amax[0] : amax[2], 8));
+        const float k1 = fmaxf(b3 ? amax[3] : amax[1], __shfl_xor_sync(0xffffffffu, b3 ? amax[1] : amax[3], 8));
+        float m = fmaxf(b2 ? k1 : k0, __shfl_xor_sync(0xffffffffu, b2 ? k0 : k1, 4));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        const float s = block_scale(m), one = 1.f / s;
+        if (!(lane & 3)) put_scale((lane >> 2) & 3, s);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) inv[c] = __shfl_sync(0xffffffffu, one, (lane & 16) + c * 4);
+    } else {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) amax[c] = fmaxf(amax[c], __shfl_xor_sync(0xffffffffu, amax[c], o));
+            const float s = block_scale(amax[c]);
+            inv[c] = 1.f / s;
+            if (!(lane & 15)) put_scale(c, s);
+        }
+    }
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
         const int col = col0 + c * 256;
-        const bool in = live && col < p.H;
-        float f[8], gg[8];
-        unpack8(v[c], f);
-        unpack8(in ? *reinterpret_cast<const uint4*>(p.g + col) : make_uint4(0, 0, 0, 0), gg);
-        float amax = 0.f;
+        if (!live || col >= p.H) continue;
+        const uint64_t inv2 = pair_of(inv[c], inv[c]);
+        uint32_t w[4], yw[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            f[e] = f[e] * rr * gg[e];
-            amax = fmaxf(amax, fabsf(f[e]));
+        for (int k = 0; k < 4; ++k) {
+            w[k] = __nv_cvt_float2_to_fp8x2(floats_of(mul2(y[c][k], inv2)), __NV_SATFINITE, __NV_E4M3);
+            const float2 f = floats_of(y[c][k]);
+            yw[k] = pack_bf16(f.x, f.y);
         }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        const float s = amax > 0.f ? amax / 448.f : 1.f, inv = 1.f / s;
-        if (in) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                w[k] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * k] * inv, f[2 * k + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-            *reinterpret_cast<uint2*>(p.q + row * p.H + col) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-            if (p.y) *reinterpret_cast<uint4*>(p.y + row * p.H + col) = pack8(f);
-            if ((lane & 15) == 0) p.scale[row * (p.H >> 7) + (col >> 7)] = s;
-        }
+        *reinterpret_cast<uint2*>(p.q + row * p.H + col) = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+        if (p.y) *reinterpret_cast<uint4*>(p.y + row * p.H + col) = make_uint4(yw[0], yw[1], yw[2], yw[3]);
     }
 }
 
@@ -134,12 +199,14 @@ CAI_API int cai_add_rmsnorm_quant(const void* x, long long ldx, const void* resi
     p.q = static_cast<__nv_fp8_storage_t*>(q);
     p.scale = scale; p.rstd = rstd;
     p.rows = rows; p.H = H; p.eps = eps;
-    const int pieces = (H + 255) / 256;
-    const int chunks = pieces <= 1 ? 1 : pieces <= 2 ? 2 : pieces <= 32 ? 4 : 8;
-    p.warps = (pieces + chunks - 1) / chunks;
+    // Four times eight columns a lane; fewer, on more warps, where the rows alone do not fill the SMs; eight beyond 8192 columns, as a CTA has eight warps.
+    const int pieces = (H + 255) / 256, sms = sm_count(current_device());
+    p.warps = pieces > 32 ? (pieces + 7) / 8 : (pieces + 3) / 4;
+    while (p.warps < 8 && p.warps < pieces && static_cast<long long>(rows) * p.warps < 8 * sms) ++p.warps;
+    const int chunks = (pieces + p.warps - 1) / p.warps;
     const int groups = 8 / p.warps;
     const unsigned grid = static_cast<unsigned>((rows + groups - 1) / groups), threads = groups * p.warps * 32;
-    const auto kernel = chunks == 1 ? add_rmsnorm_quant_kernel<1> : chunks == 2 ? add_rmsnorm_quant_kernel<2>
+    const auto kernel = chunks == 1 ? add_rmsnorm_quant_kernel<1> : chunks == 2 ? add_rmsnorm_quant_kernel<2> : chunks == 3 ? add_rmsnorm_quant_kernel<3>
                         : chunks == 4 ? add_rmsnorm_quant_kernel<4> : add_rmsnorm_quant_kernel<8>;
     const cudaError_t e = launch_early(kernel, grid, threads, 0, static_cast<cudaStream_t>(stream), p);
     if (e != cudaSuccess) {

@@ -87,6 +87,21 @@ def test_norm_of_zeros_and_of_what_is_not_finite():
     assert ops.add_rmsnorm_quant(x[:0], None, g, keep_y=True)[1].shape == (0, 256)
 
 
+def test_norm_of_very_small_rows():
+    """Blocks whose largest magnitude is 2^-120 or less beside ordinary ones: no scale whose reciprocal leaves fp32, no NaN."""
+    from cai_b200 import ops
+    x = torch.ones(3, 512, device="cuda", dtype=torch.bfloat16)
+    g = torch.ones(512, device="cuda", dtype=torch.bfloat16)
+    g[128:256] = 2.0 ** -125
+    g[256:384] = 0
+    g[300] = -2.0 ** -133
+    h, q, s, rstd, y = ops.add_rmsnorm_quant(x, None, g, keep_y=True)
+    assert torch.isfinite(q.float()).all() and torch.isfinite(s).all() and torch.isfinite(1 / s).all()
+    back = q.float() * s.repeat_interleave(128, 1)
+    # (1 + eps)^(-1/2) is the block's largest and its only value: 448 scales, within their rounding; y rounds it to 1
+    assert ((back[:, :128] - rstd[:, None]).abs() <= 2.0 ** -22).all() and (y[:, :128] == 1).all() and (back[:, 128:384].abs() <= 2.0 ** -120).all()
+
+
 def test_norm_gives_what_its_parts_give():
     """Against the norm and the quantiser of their own: the same stream and statistics, e4m3 numbers at most a step apart (their y is rounded in between)."""
     from cai_b200 import ops
