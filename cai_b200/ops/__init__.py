@@ -7,13 +7,14 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import KernelError, calls, check, device_status, lib
+from ._lib import KernelError, calls, check, device_status, lib, new_tensors
 
 EPI_BF16, EPI_F32, EPI_F32_ACCUM, EPI_BF16_RESIDUAL, EPI_SWIGLU, EPI_SWIGLU_BWD = 0, 1, 2, 3, 4, 5
 
 
 _BF16, _F32 = torch.bfloat16, torch.float32
-_current_device = _raw_stream = None
+_F8 = torch.float8_e4m3fn
+_current_device = _raw_stream = _new_tensors = None
 
 
 def _stream():
@@ -28,6 +29,14 @@ def _stream():
 
 def _p(t):
     return t.data_ptr() if t is not None else None
+
+
+def _new(like, *specs):
+    """Uninitialised tensors on like's device, one for each (dtype, size, ...), None for None."""
+    global _new_tensors
+    if _new_tensors is None:
+        _new_tensors = new_tensors()
+    return _new_tensors(like, *specs)
 
 
 def _need(ok, what):
@@ -202,11 +211,8 @@ def add_rmsnorm_quant(x, residual, g, eps=1e-6, *, keep_y=False):
         _need(residual.dtype is _BF16 and residual.shape == x.shape and sr[1] == 1, "add_rmsnorm_quant: the residual is like x")
         ldr = sr[0] if rows > 1 else 0
     stream = _stream_for("add_rmsnorm_quant", x, residual, g)
-    h = x.new_empty(rows, H) if residual is not None else None
-    y = x.new_empty(rows, H) if keep_y else None
-    q = x.new_empty(rows, H, dtype=torch.float8_e4m3fn)
-    s = x.new_empty(rows, H // 128, dtype=_F32)
-    rstd = x.new_empty(rows, dtype=_F32)
+    h, y, q, s, rstd = _new(x, (_BF16, rows, H) if residual is not None else None, (_BF16, rows, H) if keep_y else None, (_F8, rows, H),
+                            (_F32, rows, H // 128), (_F32, rows))
     check(calls().cai_add_rmsnorm_quant(x.data_ptr(), ldx, _p(residual), ldr, g.data_ptr(), _p(h), _p(y), q.data_ptr(), s.data_ptr(), rstd.data_ptr(),
                                         rows, H, float(eps), stream), "add_rmsnorm_quant")
     return (x if h is None else h), q, s, rstd, y
@@ -341,8 +347,7 @@ def flash_attn_window_fwd(qkv, B, S, nh, nkv, hd, window, sinks=0, scale=None):
     ld = _window_pitch("flash_attn_window_fwd", qkv, B, S, (nh + 2 * nkv) * hd)
     scale = hd ** -0.5 if scale is None else scale
     stream = _stream_for("flash_attn_window_fwd", qkv)
-    out = qkv.new_empty(B * S, nh * hd)
-    lse = qkv.new_empty(B, nh, S, dtype=_F32)
+    out, lse = _new(qkv, (_BF16, B * S, nh * hd), (_F32, B, nh, S))
     check(calls().cai_flash_attn_window_fwd(qkv.data_ptr(), ld, out.data_ptr(), lse.data_ptr(), B, S, nh, nkv, hd, float(scale), window, sinks, stream),
           "flash_attn_window_fwd")
     return out, lse
@@ -359,15 +364,20 @@ def flash_attn_window_bwd(qkv, out, dout, lse, B, S, nh, nkv, hd, window, sinks=
     _need(lse.dtype is _F32 and lse.shape == (B, nh, S) and lse.is_contiguous(), "flash_attn_window_bwd: lse is f32 [B, heads, S]")
     scale = hd ** -0.5 if scale is None else scale
     stream = _stream_for("flash_attn_window_bwd", qkv, out, dout, lse, dqkv, delta, scratch)
-    if dqkv is None:
-        dqkv = qkv.new_empty(B * S, cols)
-    ldq = _window_pitch("flash_attn_window_bwd", dqkv, B, S, cols)
-    if delta is None:
-        delta = lse.new_empty(B, nh, S)
-    _need(delta.dtype is _F32 and delta.numel() >= B * nh * S and delta.is_contiguous(), "flash_attn_window_bwd: delta is f32 [B, heads, S]")
+    ldq = cols
     need = calls().cai_flash_attn_window_bwd_scratch(B, S, nh, nkv, window, sinks)
+    made = _new(qkv, (_BF16, B * S, cols) if dqkv is None else None, (_F32, B, nh, S) if delta is None else None,
+                (torch.uint8, need) if scratch is None and need else None)
+    if dqkv is None:
+        dqkv = made[0]
+    else:
+        ldq = _window_pitch("flash_attn_window_bwd", dqkv, B, S, cols)
+    if delta is None:
+        delta = made[1]
+    else:
+        _need(delta.dtype is _F32 and delta.numel() >= B * nh * S and delta.is_contiguous(), "flash_attn_window_bwd: delta is f32 [B, heads, S]")
     if scratch is None:
-        scratch = qkv.new_empty(need, dtype=torch.uint8) if need else None
+        scratch = made[2]
     else:
         _need(scratch.numel() * scratch.element_size() >= need and scratch.is_contiguous(), f"flash_attn_window_bwd: the scratch has to have {need} bytes")
     check(calls().cai_flash_attn_window_bwd(qkv.data_ptr(), ld, out.data_ptr(), dout.data_ptr(), lse.data_ptr(), delta.data_ptr(), dqkv.data_ptr(), ldq,

@@ -44,14 +44,31 @@ def calls():
     Python runs), the ctypes functions of the same names. An extension that is there but cannot be loaded is an error."""
     global _calls
     if _calls is None:
-        path = _LIB_PATH.with_name("_calls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
         module = lib()
-        if path.exists():
-            loader = importlib.machinery.ExtensionFileLoader("_calls", str(path))
-            module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_calls", loader))
-            loader.exec_module(module)
-        _calls = module
+        _calls = _extension("_calls") or module
     return _calls
+
+
+def _extension(name):
+    """The extension of that name built next to the library, or None where there is none."""
+    path = _LIB_PATH.with_name(name + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+    if not path.exists():
+        return None
+    loader = importlib.machinery.ExtensionFileLoader(name, str(path))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(name, loader))
+    loader.exec_module(module)
+    return module
+
+
+def _new_by_torch(like, *specs):
+    return tuple(like.new_empty(s[1:], dtype=s[0]) if s is not None else None for s in specs)
+
+
+def new_tensors():
+    """What the ops make their results with: ``new(like, (dtype, size, ...), ...)`` gives a tuple of uninitialised tensors on like's device, None for None.
+    The extension's function, or, where it was not built, the same through torch's Python interface."""
+    module = _extension("_tensors")
+    return module.new if module is not None else _new_by_torch
 
 
 def _declare(L):

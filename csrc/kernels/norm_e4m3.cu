@@ -55,10 +55,10 @@ __device__ __forceinline__ float block_scale(float amax) { return amax > 0.f ? f
 // its instructions: hence the arithmetic on pairs, and (kChunks = 4) the four blocks' maxima reduced together: a lane that gives two of its
 // four away at the first step and one at the second is left with one, whose scale and reciprocal it computes for the sixteen.
 template <int kChunks>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512, 2)
 add_rmsnorm_quant_kernel(const NormQuantParams p) {
     grid_dep_begin();
-    __shared__ float part[8];
+    __shared__ float part[16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int grp = warp / p.warps, sub = warp - grp * p.warps, groups = (blockDim.x >> 5) / p.warps;
     const long long row = static_cast<long long>(blockIdx.x) * groups + grp;
@@ -199,15 +199,15 @@ CAI_API int cai_add_rmsnorm_quant(const void* x, long long ldx, const void* resi
     p.q = static_cast<__nv_fp8_storage_t*>(q);
     p.scale = scale; p.rstd = rstd;
     p.rows = rows; p.H = H; p.eps = eps;
-    // Four times eight columns a lane; fewer, on more warps, where the rows alone do not fill the SMs; eight beyond 8192 columns, as a CTA has eight warps.
+    // Four times eight columns a lane; fewer, on more warps, where the rows alone do not fill the SMs. A CTA has eight warps, sixteen where a row needs more.
     const int pieces = (H + 255) / 256, sms = sm_count(current_device());
-    p.warps = pieces > 32 ? (pieces + 7) / 8 : (pieces + 3) / 4;
+    p.warps = (pieces + 3) / 4;
     while (p.warps < 8 && p.warps < pieces && static_cast<long long>(rows) * p.warps < 8 * sms) ++p.warps;
     const int chunks = (pieces + p.warps - 1) / p.warps;
-    const int groups = 8 / p.warps;
+    const int groups = p.warps > 8 ? 1 : 8 / p.warps;
     const unsigned grid = static_cast<unsigned>((rows + groups - 1) / groups), threads = groups * p.warps * 32;
     const auto kernel = chunks == 1 ? add_rmsnorm_quant_kernel<1> : chunks == 2 ? add_rmsnorm_quant_kernel<2> : chunks == 3 ? add_rmsnorm_quant_kernel<3>
-                        : chunks == 4 ? add_rmsnorm_quant_kernel<4> : add_rmsnorm_quant_kernel<8>;
+                                                                                              : add_rmsnorm_quant_kernel<4>;
     const cudaError_t e = launch_early(kernel, grid, threads, 0, static_cast<cudaStream_t>(stream), p);
     if (e != cudaSuccess) {
         set_last_error("add_rmsnorm_quant launch failed: %s", cudaGetErrorString(e));
