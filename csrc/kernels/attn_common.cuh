@@ -17,32 +17,6 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return y;
 }
 
-// ---------------------------------------------------------------- a window and sinks
-// Query q sees key k if k <= q and (k > q - window or k < sinks), with 1 <= window <= S and 0 <= sinks <= S.
-struct AttnWindow {
-    int window, sinks;
-};
-// The key tiles of query tile i, in ascending order: the sinks' tiles, then those from the one that holds the first query's first key up to the diagonal.
-struct WindowKeys {
-    int diag, near, n;
-    __host__ __device__ WindowKeys(const AttnWindow& w, int i) {
-        const int reach = i * kAttnTile - w.window + 1, lo = reach > 0 ? reach / kAttnTile : 0, sink_tiles = (w.sinks + kAttnTile - 1) / kAttnTile;
-        diag = i;
-        near = i - lo + 1;
-        n = near + (sink_tiles < lo ? sink_tiles : lo);
-    }
-    __host__ __device__ int tile(int j) const { return j < n - near ? j : diag - (n - 1 - j); }
-};
-// The query tiles that key tile j is seen by through the window: j .. last.
-__host__ __device__ inline int window_last_query_tile(const AttnWindow& w, int j, int tiles) {
-    const long long last = (static_cast<long long>(j + 1) * kAttnTile + w.window - 2) / kAttnTile;
-    return last < tiles ? static_cast<int>(last) : tiles - 1;
-}
-// Is something hidden between query tile i and key tile j <= i?
-__device__ __forceinline__ bool window_masks(const AttnWindow& w, int i, int j) {
-    return i == j || ((i - j + 1) * kAttnTile > w.window && (j + 1) * kAttnTile > w.sinks);
-}
-
 // S[128,128] = Q[128,hd] * K[128,hd]^T, both operands K-major in two 64-column sub-tiles.
 __device__ __forceinline__ void issue_qk(uint32_t d_tmem, uint32_t q_smem, uint32_t k_smem, uint32_t idesc) {
 #pragma unroll

@@ -1,0 +1,50 @@
+// attn_window.cuh - what windowed attention's forward and backward kernels share: which tiles belong together, tiles of one sequence, arithmetic on pairs.
+#pragma once
+
+#include "attn_common.cuh"
+#include "f32x2.cuh"
+#include "sm100.cuh"
+
+namespace cai {
+
+// ---------------------------------------------------------------- a window and sinks
+// Query q sees key k if k <= q and (k > q - window or k < sinks), with 1 <= window <= S and 0 <= sinks <= S.
+struct AttnWindow {
+    int window, sinks;
+};
+// The key tiles of query tile i, in ascending order: the sinks' tiles, then those from the one that holds the first query's first key up to the diagonal.
+struct WindowKeys {
+    int diag, near, n;
+    __host__ __device__ WindowKeys(const AttnWindow& w, int i) {
+        const int reach = i * kAttnTile - w.window + 1, lo = reach > 0 ? reach / kAttnTile : 0, sink_tiles = (w.sinks + kAttnTile - 1) / kAttnTile;
+        diag = i;
+        near = i - lo + 1;
+        n = near + (sink_tiles < lo ? sink_tiles : lo);
+    }
+    __host__ __device__ int tile(int j) const { return j < n - near ? j : diag - (n - 1 - j); }
+};
+// The query tiles that key tile j is seen by through the window: j .. last.
+__host__ __device__ inline int window_last_query_tile(const AttnWindow& w, int j, int tiles) {
+    const long long last = (static_cast<long long>(j + 1) * kAttnTile + w.window - 2) / kAttnTile;
+    return last < tiles ? static_cast<int>(last) : tiles - 1;
+}
+// Is something hidden between query tile i and key tile j <= i?
+__device__ __forceinline__ bool window_masks(const AttnWindow& w, int i, int j) {
+    return i == j || ((i - j + 1) * kAttnTile > w.window && (j + 1) * kAttnTile > w.sinks);
+}
+
+// A tile of one sequence of a packed tensor, 128 columns from x on, in two 64-column sub-tiles. Rows past the sequence's end come as zeros.
+__device__ __forceinline__ void load_seq_tile(void* dst, const CUtensorMap* tm, uint64_t* bar, int x, int row, int b) {
+    tma_load_3d(dst, tm, bar, x, row, b);
+    tma_load_3d(static_cast<uint8_t*>(dst) + kAttnSub, tm, bar, x + 64, row, b);
+}
+// Half `half` of the keys of O[128,hd] (+)= P[128,128](TMEM, bf16 pairs) * V[128,hd].
+__device__ __forceinline__ void issue_pv_half(uint32_t d_tmem, uint32_t p_tmem, uint64_t v_desc, uint32_t idesc, int half, bool accumulate) {
+#pragma unroll
+    for (int k = 0; k < kAttnTile / 32; ++k) {
+        const int i = half * (kAttnTile / 32) + k;
+        umma_f16_ts(d_tmem, p_tmem + i * 8, v_desc + i * (2048 >> 4), idesc, (accumulate || k > 0) ? 1u : 0u);
+    }
+}
+
+}  // namespace cai

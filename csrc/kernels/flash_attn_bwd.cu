@@ -41,6 +41,7 @@
 #include <math.h>
 
 #include "attn_common.cuh"
+#include "attn_window.cuh"
 #include "cai_kernels.h"
 #include "host_common.h"
 #include "sm100.cuh"

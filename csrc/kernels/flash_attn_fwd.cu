@@ -33,15 +33,12 @@ struct AttnFwdParams {
     __nv_bfloat16* out;
     float* lse;
     int* status;
-    AttnWindow win;   // of the windowed form, where S need not fill its last tile
 };
 
 // A warp's 32 finished rows of O, each lane with one: times `inv` to bf16, through 8 KB of the query tile, which nobody reads any more, so that the warp
 // writes two whole rows at a time; from the registers every store met 32 lines. us, two CTAs to an SM,
 // before / now: 8 x 384 tokens, 12 / 4 heads 14.8 / 11.9; 8 x 256, 32 / 8 17.2 / 15.6; 16 x 384, 16 / 4 27.7 / 25.2; 4 x 1024, 16 / 8 28.2 / 26.7.
-// kCut: only the first `rows` of them are there.
-template <bool kCut>
-__device__ __forceinline__ void put_out_rows(uint32_t stage, uint32_t tO, float inv, __nv_bfloat16* out, long long ld, int lane, int rows) {
+__device__ __forceinline__ void put_out_rows(uint32_t stage, uint32_t tO, float inv, __nv_bfloat16* out, long long ld, int lane) {
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
         uint32_t v[32];
@@ -59,45 +56,28 @@ __device__ __forceinline__ void put_out_rows(uint32_t stage, uint32_t tO, float 
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int row = i * 2 + (lane >> 4), chunk = lane & 15;
-        if (kCut && row >= rows) continue;
         *reinterpret_cast<uint4*>(out + row * ld + chunk * 8) = ld_shared_v4(stage + row * 256 + ((chunk ^ (row & 7)) << 4));
     }
 }
 
 // Softmax of one query tile, whose scores arrive block by block in one buffer of tensor memory: one thread per query row (row r of
 // the tile, lane bits in tS and tO), 128 threads. Ends by writing the tile's rows of the output.
-template <bool kWindow>
 __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, int r, int nx, uint64_t* s_full, uint64_t* p_full, uint64_t* o_final,
                                              volatile int* abort_flag, const AttnFwdParams& p, int b, int h, int row_base, int q0, const uint8_t* q_tile) {
-    // A window may hide a whole row of a tile, so that its maximum starts at a finite number: exp2(-inf - m) is 0 then as well.
-    float m_used = kWindow ? -1e30f : -INFINITY, l = 0.f;
+    float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nx; ++j) {
         if (!mbar_wait_warp(s_full, j & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
         tc_fence_after();
-        const int i = q0 / kAttnTile, kt = kWindow ? WindowKeys(p.win, i).tile(j) : j;
-        const bool diag = kWindow ? window_masks(p.win, i, kt) : j == nx - 1;
-        // of a windowed tile with something hidden, the columns first < c <= last are seen, and those below `sink`
-        const int last = r + q0 - kt * kAttnTile, first = last - p.win.window, sink = p.win.sinks - kt * kAttnTile;
+        const bool diag = (j == nx - 1);
         // the whole score row (128 fp32) comes into registers with one wait and is used for both the
         // row maximum and the exponentials
         uint32_t sc[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32(tS + c * 32, sc[c]);
         tmem_ld_wait();
-        if (kWindow && diag) {
-            // hidden scores become -inf here, so that one path serves all tiles below (a select at every exponential of every tile: 8192 tokens, 32 / 8 heads,
-            // everything visible 808 -> 473 us)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const int k = c * 32 + e;
-                    if (k > last || (k <= first && k >= sink)) sc[c][e] = 0xff800000u;   // -inf
-                }
-        }
         float mx = -INFINITY;
-        if (kWindow || !diag) {
+        if (!diag) {
             float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
@@ -140,7 +120,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, int r, in
             for (int e = 0; e < 32; e += 2) {
                 float p0 = fast_exp2(fmaf(__uint_as_float(sc[c][e]), p.scale_log2, -m_used));
                 float p1 = fast_exp2(fmaf(__uint_as_float(sc[c][e + 1]), p.scale_log2, -m_used));
-                if (!kWindow && diag) {
+                if (diag) {
                     if (c * 32 + e > r) p0 = 0.f;
                     if (c * 32 + e + 1 > r) p1 = 0.f;
                 }
@@ -159,9 +139,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t tS, uint32_t tO, int r, in
         tc_fence_after();
         const float inv = 1.f / l;
         const long long ldo = static_cast<long long>(p.nh) * kAttnHD;
-        put_out_rows<kWindow>(smem_u32(q_tile) + (r >> 5) * 8192, tO, inv, p.out + (static_cast<long long>(row_base) + q0 + (r & ~31)) * ldo + h * kAttnHD, ldo,
-                              r & 31, p.S - q0 - (r & ~31));
-        if (p.lse && (!kWindow || q0 + r < p.S))
+        put_out_rows(smem_u32(q_tile) + (r >> 5) * 8192, tO, inv, p.out + (static_cast<long long>(row_base) + q0 + (r & ~31)) * ldo + h * kAttnHD, ldo, r & 31);
+        if (p.lse)
             p.lse[(static_cast<long long>(b) * p.nh + h) * p.S + q0 + r] =
                 (m_used + log2f(l)) * 0.6931471805599453f;
     }
@@ -306,7 +285,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm, const AttnFwdParams p) {
             const uint32_t lane_bits = static_cast<uint32_t>((warp & 3) * 32) << 16;
             const uint32_t tS = tmem_base + X * 128 + lane_bits;
             const uint32_t tO = tmem_base + 256 + X * 128 + lane_bits;
-            softmax_tile<false>(tS, tO, r, nx, &s_full[X], &p_full[X], &o_final[X], abort_flag, p, b, h, row_base, q0, sQ + X * kAttnTileBytes);
+            softmax_tile(tS, tO, r, nx, &s_full[X], &p_full[X], &o_final[X], abort_flag, p, b, h, row_base, q0, sQ + X * kAttnTileBytes);
         }
     }
 
@@ -529,8 +508,7 @@ attn_fwd1_kernel(const __grid_constant__ CUtensorMap tm, const AttnFwdParams p) 
             tc_fence_after();
             const float inv = 1.f / l;
             const long long ldo = static_cast<long long>(p.nh) * kAttnHD;
-            put_out_rows<false>(smem_u32(sQ) + (r >> 5) * 8192, tO, inv, p.out + (static_cast<long long>(row_base) + q0 + (r & ~31)) * ldo + h * kAttnHD, ldo,
-                                r & 31, 32);
+            put_out_rows(smem_u32(sQ) + (r >> 5) * 8192, tO, inv, p.out + (static_cast<long long>(row_base) + q0 + (r & ~31)) * ldo + h * kAttnHD, ldo, r & 31);
             if (p.lse)
                 p.lse[(static_cast<long long>(b) * p.nh + h) * p.S + q0 + r] = (m_used + log2f(l)) * 0.6931471805599453f;
         }
@@ -549,18 +527,9 @@ attn_fwd1_kernel(const __grid_constant__ CUtensorMap tm, const AttnFwdParams p) 
 // an SM and each works while the other waits. What bounds a CTA with few
 // key blocks is its own beginning and end (barriers, first loads, the output), which the other CTA of the SM now fills: 8 x 384 tokens, 12 / 4
 // heads 19.7 -> 14.7 us against two tiles in one CTA.
-// kWindow: windowed attention with sinks over sequences of any length. The tensor map has the sequences apart (rows past a sequence's end come as zeros, never
-// as the next one's), the key tiles come in the order of WindowKeys.
 // TMEM: S / P 0-127, O 128-255.
 constexpr int kAttnHalfThreads = 192;   // warp 0 TMA, warp 1 MMA, warps 2-5 softmax
 
-template <bool kWindow>
-__device__ __forceinline__ void load_half_tile(void* dst, const CUtensorMap* tm, uint64_t* bar, int x, int b, int S, int row) {
-    if constexpr (kWindow) tma_load_3d(dst, tm, bar, x, row, b);
-    else tma_load_2d(dst, tm, bar, x, b * S + row);
-}
-
-template <bool kWindow>
 __global__ void __launch_bounds__(kAttnHalfThreads, 2)
 attn_fwd_half_kernel(const __grid_constant__ CUtensorMap tm, const AttnFwdParams p) {
     extern __shared__ uint8_t smem_raw[];
@@ -587,8 +556,7 @@ attn_fwd_half_kernel(const __grid_constant__ CUtensorMap tm, const AttnFwdParams
     const int h = (lin % heads_all) % gridDim.y, b = (lin % heads_all) / gridDim.y;
     const int g = h / (p.nh / p.nkv);
     const int q0 = tile * kAttnTile;
-    const WindowKeys keys(p.win, tile);
-    const int n = kWindow ? keys.n : tile + 1;           // key blocks up to the diagonal
+    const int n = tile + 1;                              // key blocks up to the diagonal
     const int row_base = b * p.S;
     const int col_q = h * kAttnHD, col_k = (p.nh + g) * kAttnHD, col_v = (p.nh + p.nkv + g) * kAttnHD;
 
@@ -612,19 +580,19 @@ attn_fwd_half_kernel(const __grid_constant__ CUtensorMap tm, const AttnFwdParams
     if (warp == 0) {
         if (lane == 0) {
             mbar_expect_tx(q_full, kAttnTileBytes);
-            load_half_tile<kWindow>(sQ, &tm, q_full, col_q, b, p.S, q0);
-            load_half_tile<kWindow>(sQ + kAttnSub, &tm, q_full, col_q + 64, b, p.S, q0);
+            tma_load_2d(sQ, &tm, q_full, col_q, row_base + q0);
+            tma_load_2d(sQ + kAttnSub, &tm, q_full, col_q + 64, row_base + q0);
             bool ok = true;
             for (int j = 0; j < n && ok; ++j) {
-                const int kv_row = (kWindow ? keys.tile(j) : j) * kAttnTile;
+                const int kv_row = row_base + j * kAttnTile;
                 if (!mbar_wait(k_empty, (j & 1) ^ 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
                 mbar_expect_tx(k_full, kAttnTileBytes);
-                load_half_tile<kWindow>(sK, &tm, k_full, col_k, b, p.S, kv_row);
-                load_half_tile<kWindow>(sK + kAttnSub, &tm, k_full, col_k + 64, b, p.S, kv_row);
+                tma_load_2d(sK, &tm, k_full, col_k, kv_row);
+                tma_load_2d(sK + kAttnSub, &tm, k_full, col_k + 64, kv_row);
                 if (!mbar_wait(v_empty, (j & 1) ^ 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
                 mbar_expect_tx(v_full, kAttnTileBytes);
-                load_half_tile<kWindow>(sV, &tm, v_full, col_v, b, p.S, kv_row);
-                load_half_tile<kWindow>(sV + kAttnSub, &tm, v_full, col_v + 64, b, p.S, kv_row);
+                tma_load_2d(sV, &tm, v_full, col_v, kv_row);
+                tma_load_2d(sV + kAttnSub, &tm, v_full, col_v + 64, kv_row);
             }
             grid_dep_launch();
             if (!ok)
@@ -666,7 +634,7 @@ attn_fwd_half_kernel(const __grid_constant__ CUtensorMap tm, const AttnFwdParams
         }
     } else {
         const uint32_t lane_bits = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        softmax_tile<kWindow>(tmem_base + lane_bits, tmem_base + 128 + lane_bits, (warp & 3) * 32 + lane, n, s_full, p_full, o_final, abort_flag, p, b, h,
+        softmax_tile(tmem_base + lane_bits, tmem_base + 128 + lane_bits, (warp & 3) * 32 + lane, n, s_full, p_full, o_final, abort_flag, p, b, h,
                      row_base, q0, sQ);
     }
 
@@ -676,24 +644,6 @@ attn_fwd_half_kernel(const __grid_constant__ CUtensorMap tm, const AttnFwdParams
         tc_fence_after();
         tmem_dealloc(tmem_base, 256);
     }
-}
-
-template <bool kWindow>
-int launch_half(const CUtensorMap& tm, const AttnFwdParams& p, cudaStream_t stream) {
-    constexpr int smem_half = 3 * kAttnTileBytes + 1024 + 256;
-    static bool configured[64] = {};
-    const int dev = current_device();
-    if (!configured[dev & 63]) {
-        if (cudaFuncSetAttribute(attn_fwd_half_kernel<kWindow>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_half) != cudaSuccess ||
-            cudaFuncSetAttribute(attn_fwd_half_kernel<kWindow>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) !=
-                cudaSuccess) {
-            set_last_error("cudaFuncSetAttribute(attn_fwd_half) failed");
-            return CAI_K_CUDA;
-        }
-        configured[dev & 63] = true;
-    }
-    launch_early(attn_fwd_half_kernel<kWindow>, dim3((p.S + kAttnTile - 1) / kAttnTile, p.nh, p.B), kAttnHalfThreads, smem_half, stream, tm, p);
-    return CAI_K_OK;
 }
 
 }  // namespace cai
@@ -751,10 +701,20 @@ CAI_API int cai_flash_attn_fwd_variant(const void* qkv, void* out, float* lse, i
     p.out = static_cast<__nv_bfloat16*>(out);
     p.lse = lse;
     p.status = status_words(dev);
-    p.win = {};
     const int variant = force_variant ? force_variant : cai_flash_attn_fwd_form(B, S, nh, sm_count(dev));
     if (variant == 3) {
-        if (launch_half<false>(tm, p, static_cast<cudaStream_t>(stream))) return CAI_K_CUDA;
+        constexpr int smem_half = 3 * kAttnTileBytes + 1024 + 256;
+        static bool configured_half[64] = {};
+        if (!configured_half[dev & 63]) {
+            if (cudaFuncSetAttribute(attn_fwd_half_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_half) != cudaSuccess ||
+                cudaFuncSetAttribute(attn_fwd_half_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) !=
+                    cudaSuccess) {
+                set_last_error("cudaFuncSetAttribute(attn_fwd_half) failed");
+                return CAI_K_CUDA;
+            }
+            configured_half[dev & 63] = true;
+        }
+        launch_early(attn_fwd_half_kernel, dim3(S / kAttnTile, nh, B), kAttnHalfThreads, smem_half, static_cast<cudaStream_t>(stream), tm, p);
     } else if (variant == 1) {
         constexpr int smem1 = 5 * kAttnTileBytes + 1024 + 256;
         static bool configured1[64] = {};
@@ -773,28 +733,6 @@ CAI_API int cai_flash_attn_fwd_variant(const void* qkv, void* out, float* lse, i
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
         set_last_error("attn_fwd launch failed: %s", cudaGetErrorString(e));
-        return CAI_K_CUDA;
-    }
-    return CAI_K_OK;
-}
-
-CAI_API int cai_flash_attn_window_fwd(const void* qkv, long long ld, void* out, float* lse, int B, int S, int nh, int nkv, int hd, float scale,
-                                      int window, int sinks, void* stream) {
-    if (!window_call_ok("flash_attn_window_fwd", qkv, ld, out, B, S, nh, nkv, hd, scale, window, sinks)) return CAI_K_BAD_ARG;
-    if (B == 0 || S == 0) return CAI_K_OK;
-    CUtensorMap tm;
-    if (!encode_tmap_3d(&tm, qkv, static_cast<uint64_t>(nh + 2 * nkv) * hd, S, B, ld, static_cast<uint64_t>(ld) * S, 64, kAttnTile, 2)) return CAI_K_BAD_ARG;
-    AttnFwdParams p;
-    p.B = B; p.S = S; p.nh = nh; p.nkv = nkv;
-    p.scale_log2 = scale * 1.4426950408889634f;
-    p.out = static_cast<__nv_bfloat16*>(out);
-    p.lse = lse;
-    p.status = status_words(current_device());
-    p.win = {window < S ? window : S, sinks < S ? sinks : S};
-    if (launch_half<true>(tm, p, static_cast<cudaStream_t>(stream))) return CAI_K_CUDA;
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) {
-        set_last_error("flash_attn_window_fwd launch failed: %s", cudaGetErrorString(e));
         return CAI_K_CUDA;
     }
     return CAI_K_OK;

@@ -8,6 +8,7 @@
 #include <cuda_fp8.h>
 
 #include "cai_kernels.h"
+#include "f32x2.cuh"
 #include "host_common.h"
 #include "norm_kernels.cuh"
 #include "sm100.cuh"
@@ -24,27 +25,6 @@ struct NormQuantParams {
     float eps;
 };
 
-// Two fp32 numbers in one register pair; an instruction of the two takes one issue slot.
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 floats_of(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 __device__ __forceinline__ uint64_t bf16x2_pair(uint32_t v) { return pair_of(bf16_lo(v), bf16_hi(v)); }
 
 // The scale of a block whose largest magnitude is `amax`. Where 1 / scale would leave fp32's range the block is near enough to zero for a scale that does not.
