@@ -37,7 +37,8 @@ __device__ __forceinline__ void issue_pv(uint32_t d_tmem, uint32_t p_tmem, uint3
 }
 
 constexpr uint32_t kTileDesc = kAttnTileBytes >> 4;   // descriptor distance of two tiles
-// S[128,128] = A[128,hd] * B[128,hd]^T, both K-major in two 64-column sub-tiles, from ready-made descriptors.
+// S[128,128] = A[128,hd] * B[128,hd]^T, both K-major in two 64-column sub-tiles, from ready-made descriptors (fewer columns with an instruction
+// descriptor of fewer).
 __device__ __forceinline__ void issue_kk(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc) {
 #pragma unroll
     for (int k = 0; k < kAttnHD / 16; ++k) {

@@ -7,11 +7,19 @@
 
 namespace cai {
 
+// The lowest n of 32 bits, for any n.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
+
 // ---------------------------------------------------------------- a window and sinks
 // Query q sees key k if k <= q and (k > q - window or k < sinks), with 1 <= window <= S and 0 <= sinks <= S.
 struct AttnWindow {
     int window, sinks;
 };
+// How many of the `most` keys from k0 on are sinks, rounded up to 16.
+__host__ __device__ inline int seen_sinks(const AttnWindow& w, int k0, int most) {
+    const int n = (w.sinks - k0 + 15) / 16 * 16;
+    return n < most ? n : most;
+}
 // The key tiles of query tile i, in ascending order: the sinks' tiles, then those from the one that holds the first query's first key up to the diagonal.
 struct WindowKeys {
     int diag, near, n;
@@ -22,6 +30,8 @@ struct WindowKeys {
         n = near + (sink_tiles < lo ? sink_tiles : lo);
     }
     __host__ __device__ int tile(int j) const { return j < n - near ? j : diag - (n - 1 - j); }
+    // Of a sinks' tile only the first keys are seen: how many, up to what a product takes (16 at a time).
+    __host__ __device__ int width(const AttnWindow& w, int j) const { return j < n - near ? seen_sinks(w, j * kAttnTile, kAttnTile) : kAttnTile; }
 };
 // The query tiles that key tile j is seen by through the window: j .. last.
 __host__ __device__ inline int window_last_query_tile(const AttnWindow& w, int j, int tiles) {

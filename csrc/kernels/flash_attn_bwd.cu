@@ -238,9 +238,8 @@ __device__ __forceinline__ void write_staged(uint32_t stage, __nv_bfloat16* cons
 
 // Probabilities of one thread's 32 score columns, in place: exp2(s * scale_log2 - lse2). In the transposed form (dK / dV)
 // a column is a query with its own lse2; in the other (dQ) the thread's row is the query. One half (16 columns) per call.
-// kWindow: this thread's key is seen by the columns from..from + span - 1.
-template <bool kDiag, int kHalf, bool kWindow = false>
-__device__ __forceinline__ void prob_cols(uint32_t (&v)[32], const float4 (&ls)[4], float scale_log2, int r, int qb, int from = 0, int span = 0) {
+template <bool kDiag, int kHalf>
+__device__ __forceinline__ void prob_cols(uint32_t (&v)[32], const float4 (&ls)[4], float scale_log2, int r, int qb) {
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
         const float l[4] = {ls[e4].x, ls[e4].y, ls[e4].z, ls[e4].w};
@@ -249,39 +248,74 @@ __device__ __forceinline__ void prob_cols(uint32_t (&v)[32], const float4 (&ls)[
             const int e = kHalf * 16 + e4 * 4 + t;
             float pv = fast_exp2(__uint_as_float(v[e]) * scale_log2 - l[t]);
             if constexpr (kDiag) {
-                if constexpr (kWindow) {
-                    if (static_cast<unsigned>(e - from) >= static_cast<unsigned>(span)) pv = 0.f;
-                } else {
-                    if (r > qb + e) pv = 0.f;  // key (row r) may not lie after the query (column)
-                }
+                if (r > qb + e) pv = 0.f;  // key (row r) may not lie after the query (column)
             }
             v[e] = __float_as_uint(pv);
         }
     }
 }
-// kWindow: this thread's query sees the columns first < e <= last and those below `sink`.
-template <bool kDiag, bool kWindow = false>
-__device__ __forceinline__ void prob_rows(uint32_t (&v)[32], float lse2, float scale_log2, int r, int kb, int last = 0, int first = 0, int sink = 0) {
+template <bool kDiag>
+__device__ __forceinline__ void prob_rows(uint32_t (&v)[32], float lse2, float scale_log2, int r, int kb) {
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
         float pv = fast_exp2(__uint_as_float(v[e]) * scale_log2 - lse2);
         if constexpr (kDiag) {
-            if constexpr (kWindow) {
-                if (e > last || (e <= first && e >= sink)) pv = 0.f;
-            } else {
-                if (kb + e > r) pv = 0.f;
-            }
+            if (kb + e > r) pv = 0.f;
         }
         v[e] = __float_as_uint(pv);
     }
 }
+// The windowed form's, a bit of `seen` a column where `hides`, arithmetic on pairs: of half kHalf with the columns' own statistics (negated), or
+// of all with the row's.
+template <int kHalf>
+__device__ __forceinline__ void window_prob_cols(uint32_t (&v)[32], const float4 (&neg_ls)[4], float scale_log2, bool hides, uint32_t seen) {
+    const uint64_t scale2 = pair_of(scale_log2, scale_log2);
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+        const float l[4] = {neg_ls[e4].x, neg_ls[e4].y, neg_ls[e4].z, neg_ls[e4].w};
+#pragma unroll
+        for (int t = 0; t < 4; t += 2) {
+            const int e = kHalf * 16 + e4 * 4 + t;
+            const float2 x = floats_of(fma2(pair_of(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale2, pair_of(l[t], l[t + 1])));
+            v[e] = __float_as_uint(fast_exp2(x.x));
+            v[e + 1] = __float_as_uint(fast_exp2(x.y));
+        }
+    }
+    if (hides) {
+#pragma unroll
+        for (int e = kHalf * 16; e < kHalf * 16 + 16; ++e)
+            if (!(seen & (1u << e))) v[e] = 0;
+    }
+}
+__device__ __forceinline__ void window_prob_rows(uint32_t (&v)[32], float neg_lse2, float scale_log2, bool hides, uint32_t seen) {
+    const uint64_t scale2 = pair_of(scale_log2, scale_log2), l2 = pair_of(neg_lse2, neg_lse2);
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+        const float2 x = floats_of(fma2(pair_of(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), scale2, l2));
+        v[e] = __float_as_uint(fast_exp2(x.x));
+        v[e + 1] = __float_as_uint(fast_exp2(x.y));
+    }
+    if (hides) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+            if (!(seen & (1u << e))) v[e] = 0;
+    }
+}
+// Two of dS = P (dP - delta), in bf16.
+__device__ __forceinline__ uint32_t window_ds(const uint32_t p0, const uint32_t p1, const uint32_t dp0, const uint32_t dp1, float neg_d0, float neg_d1) {
+    const float2 x = floats_of(mul2(pair_of(__uint_as_float(p0), __uint_as_float(p1)),
+                                    add2(pair_of(__uint_as_float(dp0), __uint_as_float(dp1)), pair_of(neg_d0, neg_d1))));
+    return pack_bf16(x.x, x.y);
+}
 
 // D[128,hd] (+)= A[128,128](TMEM, bf16 pairs) * B[128,hd] with B MN-major in two 16 KiB sub-tiles; the A operand sits in
 // four pieces of 16 columns, 32 columns apart (each where one warp group read its 32 fp32 columns from).
-__device__ __forceinline__ void issue_pv_g16(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate) {
+// kCut: only the first `keys` (a multiple of 16) of the inner dimension.
+template <bool kCut = false>
+__device__ __forceinline__ void issue_pv_g16(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate, int keys = kAttnTile) {
 #pragma unroll
     for (int k = 0; k < kAttnTile / 16; ++k)
-        umma_f16_ts(d_tmem, a_tmem + (k >> 1) * 32 + (k & 1) * 8, b_desc + k * (2048 >> 4), idesc, (accumulate || k > 0) ? 1u : 0u);
+        if (!kCut || k * 16 < keys) umma_f16_ts(d_tmem, a_tmem + (k >> 1) * 32 + (k & 1) * 8, b_desc + k * (2048 >> 4), idesc, (accumulate || k > 0) ? 1u : 0u);
 }
 // D[128,hd] (+)= A[128,128] * B[128,hd], both in shared memory: A K-major, B MN-major.
 __device__ __forceinline__ void issue_pd_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate) {
@@ -491,14 +525,19 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
         for (int it = 0; it < iters; ++it) {
             const int i = q_first + it % per_head;
             const bool diag = kWindow ? window_masks(p.win, i, j) : it % per_head == 0;
-            const int from = kWindow ? (j - i) * kAttnTile + r - qb : 0, span = !kWindow || j * kAttnTile + r < p.win.sinks ? 0x7fffffff : p.win.window;
+            // kWindow: the 32 columns this thread's key is seen by, a bit each: from its own query on, to the window's end or, as a sink, without one
+            uint32_t seen = ~0u;
+            if (kWindow && diag) {
+                const int from = (j - i) * kAttnTile + r - qb;
+                seen = ~bits_below(from) & (j * kAttnTile + r < p.win.sinks ? ~0u : bits_below(from + p.win.window));
+            }
             const float delta = delta_next;
             if (!mbar_wait_warp(s_full, it & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
             tc_fence_after();
             uint32_t pr[32];
             tmem_ld_32x32(tSg, pr);
             __syncwarp();
-            stat[lane] = lse_next * 1.4426950408889634f;
+            stat[lane] = lse_next * (kWindow ? -1.4426950408889634f : 1.4426950408889634f);
             if (it + 1 < iters) {
                 lse_next = stat_at(p.lse, it + 1, INFINITY);
                 delta_next = stat_at(p.delta, it + 1, 0.f);
@@ -510,14 +549,16 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
             tmem_ld_wait();
             tc_fence_before();
             mbar_arrive_warp(s_empty);
-            if (diag) prob_cols<true, 0, kWindow>(pr, ls, p.scale_log2, r, qb, from, span);
+            if constexpr (kWindow) window_prob_cols<0>(pr, ls, p.scale_log2, diag, seen);
+            else if (diag) prob_cols<true, 0>(pr, ls, p.scale_log2, r, qb);
             else prob_cols<false, 0>(pr, ls, p.scale_log2, r, qb);
 #pragma unroll
             for (int e = 0; e < 4; ++e) ls[e] = reinterpret_cast<const float4*>(stat)[4 + e];
-            if (diag) prob_cols<true, 1, kWindow>(pr, ls, p.scale_log2, r, qb, from, span);
+            if constexpr (kWindow) window_prob_cols<1>(pr, ls, p.scale_log2, diag, seen);
+            else if (diag) prob_cols<true, 1>(pr, ls, p.scale_log2, r, qb);
             else prob_cols<false, 1>(pr, ls, p.scale_log2, r, qb);
             __syncwarp();
-            stat[lane] = delta;
+            stat[lane] = kWindow ? -delta : delta;
             if (it > 0 && !mbar_wait_warp(p_free, (it - 1) & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
             auto give_p = [&]() {
 #pragma unroll
@@ -542,6 +583,11 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
             for (int e4 = 0; e4 < 8; ++e4) {
                 const float4 d = reinterpret_cast<const float4*>(stat)[e4];
                 const int e = e4 * 4;
+                if constexpr (kWindow) {
+                    dk[e4 * 2] = window_ds(pr[e], pr[e + 1], dp[e], dp[e + 1], d.x, d.y);
+                    dk[e4 * 2 + 1] = window_ds(pr[e + 2], pr[e + 3], dp[e + 2], dp[e + 3], d.z, d.w);
+                    continue;
+                }
                 dk[e4 * 2] = pack_bf16(__uint_as_float(pr[e]) * (__uint_as_float(dp[e]) - d.x),
                                        __uint_as_float(pr[e + 1]) * (__uint_as_float(dp[e + 1]) - d.y));
                 dk[e4 * 2 + 1] = pack_bf16(__uint_as_float(pr[e + 2]) * (__uint_as_float(dp[e + 2]) - d.z),
@@ -707,7 +753,7 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
                 for (int k = 0; k < 32; ++k) __nanosleep(50000);
         }
     } else if (warp == 1) {
-        // ---------------- S = Q K^T, up to two steps ahead of the compute warps
+        // ---------------- S = Q K^T, up to two steps ahead of the compute warps (kWindow: sinks' tiles as wide as there are sinks, all three products)
         const uint32_t idesc_kk = umma_idesc_bf16(128, 128, 0, 0);
         const uint64_t qd = umma_smem_desc_sw128(smem_u32(sQ), 0, 1024), kd = umma_smem_desc_sw128(smem_u32(sK), 0, 1024);
         const bool leader = elect_one();
@@ -720,7 +766,7 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
                 !mbar_wait_warp(&s_empty[buf], ((j >> 1) & 1) ^ 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
             tc_fence_after();
             if (leader) {
-                issue_kk(tS + buf * 128, qd, kd + ks * kTileDesc, idesc_kk);
+                issue_kk(tS + buf * 128, qd, kd + ks * kTileDesc, kWindow ? umma_idesc_bf16(128, keys.width(p.win, j), 0, 0) : idesc_kk);
                 umma_commit(&s_full[buf]);
             }
             if (++ks == 3) {
@@ -745,7 +791,7 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
                     !mbar_wait_warp(ds_ready, (j - 1) & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
                 tc_fence_after();
                 if (leader) {
-                    issue_pv_g16(tdQ, tdP, kd + ks * kTileDesc, idesc_mn, j > 1);
+                    issue_pv_g16<kWindow>(tdQ, tdP, kd + ks * kTileDesc, idesc_mn, j > 1, kWindow ? keys.width(p.win, j - 1) : kAttnTile);
                     umma_commit(&k_empty[ks]);
                     if (j == n) umma_commit(final_bar);
                 }
@@ -758,7 +804,7 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
                 if (!mbar_wait_warp(&v_full[slot], (j >> 1) & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
                 tc_fence_after();
                 if (leader) {
-                    issue_kk(tdP, dod, vd + slot * kTileDesc, idesc_kk);
+                    issue_kk(tdP, dod, vd + slot * kTileDesc, kWindow ? umma_idesc_bf16(128, keys.width(p.win, j), 0, 0) : idesc_kk);
                     umma_commit(dp_full);
                     umma_commit(&v_empty[slot]);
                 }
@@ -785,11 +831,21 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
             tmem_ld_wait();
             tc_fence_before();
             mbar_arrive_warp(&s_empty[buf]);
-            const int kt = kWindow ? keys.tile(j) : j;
-            const int last = (i - kt) * kAttnTile + r - kb;
-            if (kWindow ? window_masks(p.win, i, kt) : j == i)
-                prob_rows<true, kWindow>(pr, lse2, p.scale_log2, r, kb, last, last - p.win.window, p.win.sinks - kt * kAttnTile - kb);
-            else prob_rows<false>(pr, lse2, p.scale_log2, r, kb);
+            if constexpr (kWindow) {
+                // the 32 columns this thread's query sees, a bit each: up to its own key, of the window or the sinks. (Past a sinks' tile's width the columns hold
+                // anything; they are not seen, and dQ does not read what becomes of them.)
+                const int kt = keys.tile(j);
+                const bool hides = window_masks(p.win, i, kt);
+                uint32_t seen = ~0u;
+                if (hides) {
+                    const int last = (i - kt) * kAttnTile + r - kb;
+                    seen = bits_below(last + 1) & (~bits_below(last + 1 - p.win.window) | bits_below(p.win.sinks - kt * kAttnTile - kb));
+                }
+                window_prob_rows(pr, -lse2, p.scale_log2, hides, seen);
+            } else {
+                if (j == i) prob_rows<true>(pr, lse2, p.scale_log2, r, kb);
+                else prob_rows<false>(pr, lse2, p.scale_log2, r, kb);
+            }
             if (!mbar_wait_warp(dp_full, j & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
             tc_fence_after();
             uint32_t dp[32], dk[16];
@@ -797,7 +853,8 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 32; e += 2)
-                dk[e >> 1] = pack_bf16(__uint_as_float(pr[e]) * (__uint_as_float(dp[e]) - dl),
+                if constexpr (kWindow) dk[e >> 1] = window_ds(pr[e], pr[e + 1], dp[e], dp[e + 1], -dl, -dl);
+                else dk[e >> 1] = pack_bf16(__uint_as_float(pr[e]) * (__uint_as_float(dp[e]) - dl),
                                        __uint_as_float(pr[e + 1]) * (__uint_as_float(dp[e + 1]) - dl));
             tmem_st_32x16(tdPg, dk);
             tmem_st_wait();

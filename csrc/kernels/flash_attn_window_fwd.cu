@@ -77,9 +77,6 @@ __device__ __forceinline__ void put_window_rows(uint32_t stage, uint32_t tO, flo
 }
 
 
-// The lowest n of 64 bits, for any n.
-__device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
-
 // The blocks of 64 keys of query tile i, in ascending order: those of the sinks, then from the one with the first query's first key to the one with the last
 // query.
 struct WindowBlocks {
@@ -125,14 +122,20 @@ struct WindowStream {
 // What the issuing warp has to know of it: how many blocks the item has left. (With the whole stream it spent 240 cycles a block on it, 700 an item, beside an idle
 // pipe.)
 struct WindowCount {
-    int round, left, n;
+    int round, left, n, sinks;
     __device__ WindowCount(const WindowFwdParams& p) : round(-1) { next_item(p); }
     __device__ bool there() const { return left > 0; }
     __device__ bool first() const { return left == n; }
+    // keys of block u of the item, as products take them
+    __device__ int width(const WindowFwdParams& p, int u) const { return u < sinks ? seen_sinks(p.win, u * kBlock, kBlock) : kBlock; }
     __device__ void next_item(const WindowFwdParams& p) {
         ++round;
         const int item = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        left = n = item < p.items ? WindowBlocks(p.win, p.tiles - 1 - p.heads_all.quotient(item), p.S).n : 0;
+        left = n = 0;
+        if (item >= p.items) return;
+        const WindowBlocks blocks(p.win, p.tiles - 1 - p.heads_all.quotient(item), p.S);
+        left = n = blocks.n;
+        sinks = blocks.sinks;
     }
     __device__ __forceinline__ void next(const WindowFwdParams& p) {
         if (--left == 0) next_item(p);
@@ -219,17 +222,20 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tm, const WindowFwdPa
         // S runs two blocks ahead: S of block c + 2 goes out behind P V of block c, whose P it overwrites (the pipe keeps their order). The issuing thread is at
         // most one MMA ahead of the pipe, which idles while the thread waits (some 200 cycles for a barrier that is satisfied already) or commits (100
         // to 150): a block has two waits and one commit.
-        const uint32_t idesc_qk = umma_idesc_bf16(128, kBlock, 0, 0), idesc_pv = umma_idesc_bf16(128, 128, 0, 1);
+        const uint32_t idesc_pv = umma_idesc_bf16(128, 128, 0, 1);
         const uint64_t qd = umma_smem_desc_sw128(smem_u32(sQ), 0, 1024), kd = umma_smem_desc_sw128(smem_u32(sK), 0, 1024);
         const uint64_t vd = umma_smem_desc_sw128(smem_u32(sV), kBlockSub, 1024);
         const uint32_t tS = tmem_base, tO = tmem_base + 128;
         const bool leader = elect_one();
-        auto scores = [&](int slot) {
+        auto scores = [&](int slot, uint32_t idesc_qk) {
 #pragma unroll
             for (int k = 0; k < kAttnHD / 16; ++k)
                 umma_f16_ss(tS + slot * kBlock, qd + (((k >> 2) * kAttnSub + (k & 3) * 32) >> 4),
                             kd + ((slot * kBlockBytes + (k >> 2) * kBlockSub + (k & 3) * 32) >> 4), idesc_qk, k > 0 ? 1u : 0u);
         };
+        // A sinks' block is as wide as there are sinks: 3 to 4 % of the products with windows of a thousand.
+        constexpr uint32_t idesc_full = umma_idesc_bf16(128, kBlock, 0, 0);
+        auto idesc_of = [&](const WindowCount& at, int u) { return u < at.sinks ? umma_idesc_bf16(128, at.width(p, u), 0, 0) : idesc_full; };
         uint32_t q_phase = 0, o_phase = 1;      // o_empty: nothing to wait for before the first item
         // the queries of the next item's first block
         auto queries = [&]() {
@@ -240,13 +246,13 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tm, const WindowFwdPa
         };
         WindowCount cur(p), ahead = cur;
         bool ok = true;
-        for (int c = 0; c < 2 && ahead.there() && ok; ++c) {
+        for (int k = 0; k < 2 && ahead.there() && ok; ++k) {
             ok = (!ahead.first() || queries()) && mbar_wait_warp(k_first, 0, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN);
             if (!ok) break;
             tc_fence_after();
             if (leader) {
-                scores(c);
-                umma_commit(&done[c]);
+                scores(k, idesc_of(ahead, ahead.n - ahead.left));
+                umma_commit(&done[k]);
             }
             __syncwarp();
             ahead.next(p);
@@ -268,16 +274,29 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tm, const WindowFwdPa
             for (int k = 0; k < kBlock / 16; ++k)
                 umma_f16_ts(tO, tS + (c & 1) * kBlock + k * 8, vd + (((c & 1) * kBlockBytes + k * 2048) >> 4), idesc_pv, (!first || k > 0) ? 1u : 0u);
         };
+        auto weigh_sinks = [&](bool first, int width) {
+            for (int k = 0; k * 16 < width; ++k)
+                umma_f16_ts(tO, tS + (c & 1) * kBlock + k * 8, vd + (((c & 1) * kBlockBytes + k * 2048) >> 4), idesc_pv, (!first || k > 0) ? 1u : 0u);
+        };
         while (cur.there() && ok) {
             const int n = cur.n;
             int u = 0;
             // while the block two ahead is of the same item nothing else has to be known
-            for (; u + 2 < n; ++u, ++c) {
+            for (; u + 2 < n && u < cur.sinks; ++u, ++c) {
+                if (!(ok = come(u == 0))) break;
+                if (leader) {
+                    weigh_sinks(u == 0, cur.width(p, u));
+                    scores(c & 1, idesc_of(cur, u + 2));
+                    umma_commit(&done[c & 1]);     // step c + 2
+                }
+                __syncwarp();
+            }
+            for (; u + 2 < n && ok; ++u, ++c) {
                 if (!(ok = come(u == 0))) break;
                 if (leader) {
                     weigh(u == 0);
-                    scores(c & 1);
-                    umma_commit(&done[c & 1]);     // step c + 2
+                    scores(c & 1, idesc_full);
+                    umma_commit(&done[c & 1]);
                 }
                 __syncwarp();
             }
@@ -286,16 +305,17 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tm, const WindowFwdPa
                 const bool more = ahead.there(), turn = more && ahead.first();
                 if (!(ok = come(u == 0))) break;
                 if (leader) {
-                    weigh(u == 0);
+                    if (u < cur.sinks) weigh_sinks(u == 0, cur.width(p, u));
+                    else weigh(u == 0);
                     if (u + 1 == n) umma_commit(o_full);
-                    if (more && !turn) scores(c & 1);
+                    if (more && !turn) scores(c & 1, idesc_of(ahead, ahead.n - ahead.left));
                     if (!turn) umma_commit(&done[c & 1]);
                 }
                 __syncwarp();
                 if (turn) {
                     if (!(ok = queries())) break;
                     if (leader) {
-                        scores(c & 1);
+                        scores(c & 1, idesc_of(ahead, 0));
                         umma_commit(&done[c & 1]);
                     }
                     __syncwarp();
@@ -323,11 +343,13 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tm, const WindowFwdPa
                 const uint32_t tS = tmem_base + (c & 1) * kBlock + lane_bits;
                 const int k0 = at.keys.block(u) * kBlock;
                 const bool hides = k0 + kBlock > q0 || (q0 + kAttnTile - k0 > p.win.window && k0 + kBlock > p.win.sinks);
-                uint64_t seen = ~0ull;
+                uint32_t seen[2] = {~0u, ~0u};
                 if (hides) {
-                    // Seen are the columns before < k <= last and those below `sink`; a bit each.
+                    // seen are the columns before < k <= last and those below `sink`; a bit each
                     const int last = r + q0 - k0, before = last - p.win.window, sink = p.win.sinks - k0;
-                    seen = (bits_below(last + 1) & ~bits_below(before + 1)) | (bits_below(sink) & bits_below(last + 1));
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        seen[h] = bits_below(last + 1 - h * 32) & (~bits_below(before + 1 - h * 32) | bits_below(sink - h * 32));
                 }
                 if (!mbar_wait_warp(&done[c & 1], (c >> 1) & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
                 tc_fence_after();
@@ -340,10 +362,9 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tm, const WindowFwdPa
                     // heads, everything visible 808 -> 473 us).
 #pragma unroll
                     for (int c2 = 0; c2 < 2; ++c2) {
-                        const uint32_t word = static_cast<uint32_t>(seen >> (c2 * 32));
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (!(word & (1u << e))) sc[c2][e] = 0xff800000u;   // -inf
+                            if (!(seen[c2] & (1u << e))) sc[c2][e] = 0xff800000u;   // -inf
                     }
                 }
                 float mx[8];
@@ -366,13 +387,13 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tm, const WindowFwdPa
                         if (!mbar_wait_warp(&done[(c + 1) & 1], ((c + 1) >> 1) & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
                         tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < 8; ++c) {
+                        for (int o = 0; o < 8; ++o) {
                             uint32_t v[16];
-                            tmem_ld_32x16(tO + c * 16, v);
+                            tmem_ld_32x16(tO + o * 16, v);
                             tmem_ld_wait();
 #pragma unroll
                             for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
-                            tmem_st_32x16(tO + c * 16, v);
+                            tmem_st_32x16(tO + o * 16, v);
                         }
                         tmem_st_wait();
                     }
@@ -380,18 +401,18 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tm, const WindowFwdPa
                 }
                 const uint64_t m2 = pair_of(-m_used, -m_used);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int half = 0; half < 2; ++half) {
                     uint32_t pk[16];
                     uint64_t s2 = 0;
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
-                        const float2 x = floats_of(fma2(pair_of(__uint_as_float(sc[c][e]), __uint_as_float(sc[c][e + 1])), scale2, m2));
+                        const float2 x = floats_of(fma2(pair_of(__uint_as_float(sc[half][e]), __uint_as_float(sc[half][e + 1])), scale2, m2));
                         const float w0 = fast_exp2(x.x), w1 = fast_exp2(x.y);
                         s2 = add2(s2, pair_of(w0, w1));
                         pk[e >> 1] = pack_bf16(w0, w1);
                     }
                     l2 = add2(l2, s2);
-                    tmem_st_32x16(tS + c * 16, pk);
+                    tmem_st_32x16(tS + half * 16, pk);
                 }
                 tmem_st_wait();
                 tc_fence_before();
