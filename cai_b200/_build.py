@@ -90,7 +90,7 @@ def build_kernels(verbose=False, ptxas_info=False) -> Path:
     if jobs or _newer(lib, objs):
         _run([NVCC, "-shared", "-o", lib] + objs + ["-cudart", "static", "-ldl", "-lpthread"], verbose)
     build_calls(verbose)
-    build_tensors(verbose)
+    build_ops(verbose)
     # stand-alone CUDA tools (measurement programs that need no Python): bin/<name>
     BINDIR.mkdir(parents=True, exist_ok=True)
     for t in sorted((CSRC / "tools").glob("*.cu")):
@@ -114,20 +114,20 @@ def build_calls(verbose=False):
     return out
 
 
-def build_tensors(verbose=False):
-    """The ops' results as torch tensors (lib/_tensors.<abi>.so). Without Python's headers or torch's there is none, and the ops go through torch's
-    Python interface."""
+def build_ops(verbose=False):
+    """Operators on torch tensors as a Python extension (lib/_ops.<abi>.so): those whose arguments are checked and whose results are made in native code.
+    Needs Python's headers and torch's."""
     include = Path(sysconfig.get_paths()["include"])
     spec = importlib.util.find_spec("torch")
-    src, out = CSRC / "python" / "tensors.cc", LIBDIR / ("_tensors" + sysconfig.get_config_var("EXT_SUFFIX"))
+    src, out = CSRC / "python" / "ops.cc", LIBDIR / ("_ops" + sysconfig.get_config_var("EXT_SUFFIX"))
     torch = Path(spec.origin).parent if spec and spec.origin else None
     if torch is None or not (include / "Python.h").exists() or not (torch / "include" / "ATen" / "cuda" / "EmptyTensor.h").exists():
         return None
-    if _newer(out, [src, torch / "version.py"]):
+    if _newer(out, [src, CSRC / "kernels" / "cai_kernels.h", torch / "version.py"]):
         cuda = Path(NVCC).resolve().parent.parent / "include"
-        _run([CXX, "-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden", "-shared", "-isystem", include, "-isystem", torch / "include", "-isystem",
-              torch / "include" / "torch" / "csrc" / "api" / "include", "-isystem", cuda, src, "-o", out, "-L", torch / "lib", "-lc10", "-ltorch_cpu",
-              "-ltorch_cuda", "-ltorch_python"], verbose)
+        _run([CXX, "-std=c++17", "-O2", "-fPIC", "-fvisibility=hidden", "-Wall", "-shared", "-isystem", include, "-isystem", torch / "include", "-isystem",
+              torch / "include" / "torch" / "csrc" / "api" / "include", "-isystem", cuda, src, "-o", out, "-L", LIBDIR, "-lcai_kernels", "-L",
+              torch / "lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], verbose)
     return out
 
 

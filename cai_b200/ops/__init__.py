@@ -7,14 +7,13 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import KernelError, calls, check, device_status, lib, new_tensors
+from ._lib import KernelError, calls, check, device_status, lib, native
 
 EPI_BF16, EPI_F32, EPI_F32_ACCUM, EPI_BF16_RESIDUAL, EPI_SWIGLU, EPI_SWIGLU_BWD = 0, 1, 2, 3, 4, 5
 
 
 _BF16, _F32 = torch.bfloat16, torch.float32
-_F8 = torch.float8_e4m3fn
-_current_device = _raw_stream = _new_tensors = None
+_current_device = _raw_stream = None
 
 
 def _stream():
@@ -29,28 +28,6 @@ def _stream():
 
 def _p(t):
     return t.data_ptr() if t is not None else None
-
-
-def _new(like, *specs):
-    """Uninitialised tensors on like's device, one for each (dtype, size, ...), None for None."""
-    global _new_tensors
-    if _new_tensors is None:
-        _new_tensors = new_tensors()
-    return _new_tensors(like, *specs)
-
-
-def _need(ok, what):
-    if not ok:
-        raise KernelError(what)
-
-
-def _stream_for(what, *tensors):
-    """The stream of a call on these tensors, which have to be the current device's: a launch goes to that device's current stream."""
-    stream, device = _stream(), _current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != device:
-            raise KernelError(f"{what}: a tensor on {t.device}, and cuda:{device} is the current device")
-    return stream
 
 
 def gemm(a, b, *, trans_a=False, trans_b=False, out=None, out_dtype=torch.bfloat16, accumulate=False,
@@ -199,23 +176,7 @@ def add_rmsnorm_quant(x, residual, g, eps=1e-6, *, keep_y=False):
     ``(h, q, s, rstd, y)``: ``h`` bf16 (``x`` itself where ``residual`` is None), ``q`` e4m3 ``[rows, H]``, ``s`` f32 ``[rows, H / 128]``, ``rstd`` f32
     ``[rows]``, ``y`` bf16, or None without ``keep_y`` (a weight gradient reads it). ``q`` is rounded once, from y in fp32. The gradients are
     ``rmsnorm_bwd(h, g, rstd, dy, dx=dh, dx_accumulate=True)``: ``dh``, the gradient of ``h`` that comes past the norm, becomes that of x and of residual."""
-    _need(x.dtype is _BF16 and g.dtype is _BF16 and x.dim() == 2, "add_rmsnorm_quant: x is bf16 [rows, H], g bf16 [H]")
-    rows, H = x.shape
-    sx = x.stride()
-    _need(g.shape == (H,) and g.is_contiguous(), "add_rmsnorm_quant: g has one element a column")
-    _need(sx[1] == 1, "add_rmsnorm_quant: rows of x have to be contiguous")
-    ldx = sx[0] if rows > 1 else 0
-    ldr = 0
-    if residual is not None:
-        sr = residual.stride()
-        _need(residual.dtype is _BF16 and residual.shape == x.shape and sr[1] == 1, "add_rmsnorm_quant: the residual is like x")
-        ldr = sr[0] if rows > 1 else 0
-    stream = _stream_for("add_rmsnorm_quant", x, residual, g)
-    h, y, q, s, rstd = _new(x, (_BF16, rows, H) if residual is not None else None, (_BF16, rows, H) if keep_y else None, (_F8, rows, H),
-                            (_F32, rows, H // 128), (_F32, rows))
-    check(calls().cai_add_rmsnorm_quant(x.data_ptr(), ldx, _p(residual), ldr, g.data_ptr(), _p(h), _p(y), q.data_ptr(), s.data_ptr(), rstd.data_ptr(),
-                                        rows, H, float(eps), stream), "add_rmsnorm_quant")
-    return (x if h is None else h), q, s, rstd, y
+    return native().add_rmsnorm_quant(x, residual, g, eps, keep_y)
 
 
 def rope_table(seq, hd, theta=10000.0, device="cuda"):
@@ -245,21 +206,7 @@ def rope_apply_axes_(qkv, freqs, pos, nh, nkv, hd, sections, *, interleaved=Fals
     ``freqs`` f64 ``[hd / 2]`` (:func:`rope_freqs`); ``sections``: the axes' numbers of pairs, which add up to ``hd / 2``. They follow one another, or,
     ``interleaved``, pair i belongs to axis ``i % axes`` as long as that axis has pairs left, and to axis 0 after that (refused where an axis would not
     get its number). ``inverse`` turns back: the backward pass. ``hd`` a multiple of 16 up to 256."""
-    sections = tuple(sections)
-    axes = len(sections)
-    _need(qkv.dtype is _BF16 and qkv.dim() == 2 and qkv.stride(1) == 1, "rope_apply_axes_: qkv is bf16 [T, columns] with contiguous rows")
-    T, cols = qkv.shape
-    _need(cols >= (nh + nkv) * hd, "rope_apply_axes_: qkv holds fewer columns than its q and k heads")
-    _need(T < 2 or qkv.stride(0) >= cols, "rope_apply_axes_: rows of qkv overlap")
-    _need(1 <= axes <= 4 and pos.dtype is torch.int32 and pos.shape == (axes, T), "rope_apply_axes_: pos is int32 [axes, T], with one to four axes")
-    _need(pos.stride(1) == 1 or T < 2, "rope_apply_axes_: an axis' positions have to be contiguous")
-    _need(freqs.dtype is torch.float64 and freqs.shape == (hd // 2,) and freqs.is_contiguous(), "rope_apply_axes_: freqs is f64 [hd / 2]")
-    n = sections + (0,) * (4 - axes)
-    ld = qkv.stride(0) if T > 1 else (cols + 7) // 8 * 8
-    ldp = pos.stride(0) if axes > 1 else T
-    check(calls().cai_rope_apply_axes(qkv.data_ptr(), freqs.data_ptr(), pos.data_ptr(), ldp, T, nh, nkv, hd, ld, axes, n[0], n[1], n[2], n[3],
-                                      int(interleaved), int(inverse), _stream_for("rope_apply_axes_", qkv, freqs, pos)), "rope_apply_axes_")
-    return qkv
+    return native().rope_apply_axes_(qkv, freqs, pos, nh, nkv, hd, sections, interleaved, inverse)
 
 
 def swiglu_fwd(gu):
@@ -332,57 +279,18 @@ def flash_attn_bwd(qkv, out, dout, lse, B, S, nh, nkv, hd, scale=None, dqkv=None
     return dqkv
 
 
-def _window_pitch(what, t, B, S, cols):
-    """Row pitch of a packed [B * S, cols] bf16 tensor."""
-    _need(t.dtype is _BF16 and t.shape == (B * S, cols), f"{what}: needs bf16 [B * S, (heads + 2 kv_heads) * head_dim]")
-    st = t.stride()
-    _need(st[1] == 1 and (B * S < 2 or st[0] >= cols), f"{what}: rows have to be contiguous and apart")
-    return st[0] if B * S > 1 else cols
-
-
 def flash_attn_window_fwd(qkv, B, S, nh, nkv, hd, window, sinks=0, scale=None):
     """Causal GQA flash attention with a window and sinks over packed ``qkv`` ``[B*S, (nh + 2 nkv) * hd]`` (bf16, any row pitch that is a multiple of 8): query i
     sees key j if ``j <= i`` and (``j > i - window`` or ``j < sinks``). Any ``S``; ``window >= 1``, ``sinks >= 0``, head_dim 128. Returns ``out`` bf16
     ``[B*S, nh * hd]`` and ``lse`` f32 ``[B, nh, S]``."""
-    ld = _window_pitch("flash_attn_window_fwd", qkv, B, S, (nh + 2 * nkv) * hd)
-    scale = hd ** -0.5 if scale is None else scale
-    stream = _stream_for("flash_attn_window_fwd", qkv)
-    out, lse = _new(qkv, (_BF16, B * S, nh * hd), (_F32, B, nh, S))
-    check(calls().cai_flash_attn_window_fwd(qkv.data_ptr(), ld, out.data_ptr(), lse.data_ptr(), B, S, nh, nkv, hd, float(scale), window, sinks, stream),
-          "flash_attn_window_fwd")
-    return out, lse
+    return native().flash_attn_window_fwd(qkv, B, S, nh, nkv, hd, window, sinks, scale)
 
 
 def flash_attn_window_bwd(qkv, out, dout, lse, B, S, nh, nkv, hd, window, sinks=0, scale=None, dqkv=None, delta=None, scratch=None):
     """Gradient of :func:`flash_attn_window_fwd` with respect to ``qkv``, packed like it (``dqkv``, made where it is None). ``out`` and ``lse`` are the forward
     pass's, ``dout`` the gradient of ``out``. ``delta`` (f32 ``[B, nh, S]``) and ``scratch`` (uint8, :func:`flash_attn_window_bwd_scratch` bytes) are
     workspaces, made where they are None; calls that may overlap need their own. The same bits in every run."""
-    cols = (nh + 2 * nkv) * hd
-    ld = _window_pitch("flash_attn_window_bwd", qkv, B, S, cols)
-    for t in (out, dout):
-        _need(t.dtype is _BF16 and t.shape == (B * S, nh * hd) and t.is_contiguous(), "flash_attn_window_bwd: out and dout are bf16 [B * S, heads * head_dim]")
-    _need(lse.dtype is _F32 and lse.shape == (B, nh, S) and lse.is_contiguous(), "flash_attn_window_bwd: lse is f32 [B, heads, S]")
-    scale = hd ** -0.5 if scale is None else scale
-    stream = _stream_for("flash_attn_window_bwd", qkv, out, dout, lse, dqkv, delta, scratch)
-    ldq = cols
-    need = calls().cai_flash_attn_window_bwd_scratch(B, S, nh, nkv, window, sinks)
-    made = _new(qkv, (_BF16, B * S, cols) if dqkv is None else None, (_F32, B, nh, S) if delta is None else None,
-                (torch.uint8, need) if scratch is None and need else None)
-    if dqkv is None:
-        dqkv = made[0]
-    else:
-        ldq = _window_pitch("flash_attn_window_bwd", dqkv, B, S, cols)
-    if delta is None:
-        delta = made[1]
-    else:
-        _need(delta.dtype is _F32 and delta.numel() >= B * nh * S and delta.is_contiguous(), "flash_attn_window_bwd: delta is f32 [B, heads, S]")
-    if scratch is None:
-        scratch = made[2]
-    else:
-        _need(scratch.numel() * scratch.element_size() >= need and scratch.is_contiguous(), f"flash_attn_window_bwd: the scratch has to have {need} bytes")
-    check(calls().cai_flash_attn_window_bwd(qkv.data_ptr(), ld, out.data_ptr(), dout.data_ptr(), lse.data_ptr(), delta.data_ptr(), dqkv.data_ptr(), ldq,
-                                            _p(scratch), B, S, nh, nkv, hd, float(scale), window, sinks, stream), "flash_attn_window_bwd")
-    return dqkv
+    return native().flash_attn_window_bwd(qkv, out, dout, lse, B, S, nh, nkv, hd, window, sinks, scale, dqkv, delta, scratch)
 
 
 def flash_attn_window_bwd_scratch(B, S, nh, nkv, window, sinks=0):

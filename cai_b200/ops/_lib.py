@@ -16,6 +16,7 @@ from pathlib import Path
 _LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libcai_kernels.so"
 _lib = None
 _calls = None
+_native = None
 
 
 class GemmCall(ctypes.Structure):
@@ -60,15 +61,18 @@ def _extension(name):
     return module
 
 
-def _new_by_torch(like, *specs):
-    return tuple(like.new_empty(s[1:], dtype=s[0]) if s is not None else None for s in specs)
-
-
-def new_tensors():
-    """What the ops make their results with: ``new(like, (dtype, size, ...), ...)`` gives a tuple of uninitialised tensors on like's device, None for None.
-    The extension's function, or, where it was not built, the same through torch's Python interface."""
-    module = _extension("_tensors")
-    return module.new if module is not None else _new_by_torch
+def native():
+    """The operators that are native from their arguments on (module _ops). The build leaves it out where there are no Python or torch headers; without it
+    those operators are refused."""
+    global _native
+    if _native is None:
+        lib()
+        module = _extension("_ops")
+        if module is None:
+            raise KernelError("this operator needs the extension _ops, which was built without: it takes Python's and torch's headers (python -m cai_b200._build)")
+        module.bind(KernelError)
+        _native = module
+    return _native
 
 
 def _declare(L):

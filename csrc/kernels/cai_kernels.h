@@ -183,7 +183,7 @@ CAI_API int cai_rope_apply(void* qkv, const float* table, int T, int seq, int nh
                            long long ld, int inverse, void* stream);
 
 /* The same by the positions of `axes` (1 to 4) axes: pair i of a head, its elements i and i + hd / 2, is turned by
- * pos[axis(i) * ldp + row] * freqs[i] radians (any int; the product is taken in 64 bits). axis(i): the first n0 pairs belong to axis 0, the next n1 to axis 1
+ * pos[axis(i) * ldp + row] * freqs[i] radians (any int, ldp >= 0; the product is taken in 64 bits). axis(i): the first n0 pairs belong to axis 0, the next n1 to axis 1
  * and so on (the rest of the n are 0); interleaved, pair i belongs to axis i % axes while i / axes < n of that axis, and to axis 0 otherwise
  * (refused where an axis would not get its n). n0 + n1 + n2 + n3 = hd / 2, hd a multiple of 16 up to 256. */
 CAI_API int cai_rope_apply_axes(void* qkv, const double* freqs, const int* pos, long long ldp, int T, int nh, int nkv, int hd, long long ld, int axes,

@@ -128,8 +128,8 @@ CAI_API int cai_rope_apply_axes(void* qkv, const double* freqs, const int* pos, 
             set_last_error("rope_apply_axes: section %d of %d pairs does not fit every %d-th of %d pairs", a, n[a], axes, half);
             return CAI_K_BAD_ARG;
         }
-    if ((ld & 7) || ld < static_cast<long long>(nh + nkv) * hd || (reinterpret_cast<uintptr_t>(qkv) & 15) || (axes > 1 && ldp < T)) {
-        set_last_error("rope_apply_axes: rows have to start on 16 bytes and hold the q and k heads, positions to lie axis by axis");
+    if ((ld & 7) || ld < static_cast<long long>(nh + nkv) * hd || (reinterpret_cast<uintptr_t>(qkv) & 15) || ldp < 0) {
+        set_last_error("rope_apply_axes: rows have to start on 16 bytes and hold the q and k heads");
         return CAI_K_BAD_ARG;
     }
     if ((nh + nkv) * (half / 8) >= 65536) {

@@ -153,7 +153,7 @@ def _rope(**change):
 
 
 @pytest.mark.parametrize("change", [dict(hd=120), dict(hd=272), dict(hd=0), dict(axes=0), dict(axes=5), dict(n0=15), dict(n3=1, n0=15), dict(n0=-8, n1=48), dict(ld=380),
-                                    dict(ld=376), dict(qkv=P + 2), dict(ldp=9), dict(T=-1), dict(interleaved=1)], ids=str)
+                                    dict(ld=376), dict(qkv=P + 2), dict(ldp=-1), dict(T=-1), dict(interleaved=1)], ids=str)
 def test_rope_launcher_refuses(change):
     from cai_b200.ops import KernelError, calls, check
     with pytest.raises(KernelError, match="rope_apply_axes"):
@@ -191,6 +191,39 @@ def test_norm_call_refuses_tensors_that_do_not_fit():
               (x, torch.zeros(256, 4, dtype=torch.bfloat16).t(), g)):
         with pytest.raises(ops.KernelError, match="add_rmsnorm_quant"):
             ops.add_rmsnorm_quant(*a)
+
+
+def test_arguments_that_are_no_tensors_or_numbers():
+    from cai_b200 import ops
+    qkv = torch.zeros(4, 512, dtype=torch.bfloat16)
+    with pytest.raises(ops.KernelError, match="tensor"):
+        ops.flash_attn_window_fwd([1.0], 1, 4, 2, 1, 128, 4)
+    with pytest.raises(ops.KernelError, match="tensor"):
+        ops.add_rmsnorm_quant(qkv, qkv, None)
+    with pytest.raises(TypeError):
+        ops.flash_attn_window_fwd(qkv, 1, "4", 2, 1, 128, 4)
+    with pytest.raises(TypeError):
+        ops.rope_apply_axes_(qkv, torch.zeros(64, dtype=torch.float64), torch.zeros(1, 4, dtype=torch.int32), 2, 1, 128, 64)
+    with pytest.raises(ops.KernelError, match="out of range"):
+        ops.flash_attn_window_fwd(qkv, 1, 2 ** 40, 2, 1, 128, 4)
+
+
+def test_tensors_of_the_host_are_refused():
+    from cai_b200 import ops
+    x = torch.zeros(4, 512, dtype=torch.bfloat16)
+    for call in (lambda: ops.add_rmsnorm_quant(x, None, x[0]), lambda: ops.flash_attn_window_fwd(x, 1, 4, 2, 1, 128, 4),
+                 lambda: ops.rope_apply_axes_(x, torch.zeros(64, dtype=torch.float64), torch.zeros(1, 4, dtype=torch.int32), 2, 1, 128, (64,)),
+                 lambda: ops.flash_attn_window_bwd(x, x[:, :256].clone(), x[:, :256].clone(), torch.zeros(1, 2, 4), 1, 4, 2, 1, 128, 4)):
+        with pytest.raises(ops.KernelError, match="current device"):
+            call()
+
+
+def test_a_build_without_the_extension_refuses(monkeypatch):
+    from cai_b200.ops import _lib
+    monkeypatch.setattr(_lib, "_native", None)
+    monkeypatch.setattr(_lib, "_extension", lambda name: None)
+    with pytest.raises(_lib.KernelError, match="_ops"):
+        _lib.native()
 
 
 def test_frequencies():

@@ -190,6 +190,16 @@ def test_rope_axes_of_views():
     assert torch.equal(big, kept)
 
 
+def test_rope_axes_of_one_row_of_positions_for_all():
+    from cai_b200 import ops
+    qkv = torch.randn(9, 512, device="cuda").to(torch.bfloat16)
+    pos = torch.arange(100, 109, device="cuda", dtype=torch.int32)[None].expand(3, 9)
+    a, b = qkv.clone(), qkv.clone()
+    ops.rope_apply_axes_(a, ops.rope_freqs(128), pos, 2, 1, 128, [16, 24, 24])
+    ops.rope_apply_axes_(b, ops.rope_freqs(128), pos[:1].contiguous(), 2, 1, 128, [64])
+    assert torch.equal(a, b) and not torch.equal(a, qkv)
+
+
 def test_rope_axes_is_the_one_axis_rotation():
     """One axis with position t mod seq: what rope_apply_ does with its table, as near as that table's angles are."""
     from cai_b200 import ops
