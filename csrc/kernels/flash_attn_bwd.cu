@@ -49,11 +49,11 @@
 namespace cai {
 
 // How the dK / dV part of the windowed form is cut into CTAs. A key tile's sum runs over the query heads of its group and over the query tiles that see it: those of
-// the window, and, where it holds sinks, all later ones. The heads are cut into `head_parts`, the later query tiles into `far_parts` of
-// `far_tiles` each. Tiles with more than one part leave sums in fp32 in the caller's scratch, 128 KB a part, which a
+// the window, and, where it holds sinks, all later ones. The heads are cut into `head_parts`, the window's query tiles into `near_parts` of `near_tiles`
+// each, the later ones into `far_parts` of `far_tiles`. Tiles with more than one part leave sums in fp32 in the caller's scratch, 128 KB a part, which a
 // second kernel adds up in a fixed order.
 struct AttnWindowParts {
-    int head_parts, far_parts, far_tiles;
+    int head_parts, near_parts, near_tiles, far_parts, far_tiles;
     int sink_tiles;          // key tiles that hold sinks and are seen by query tiles behind their window
     int near_ctas, far_ctas, near_slots;
 };
@@ -61,21 +61,22 @@ struct AttnWindowParts {
 // The part that CTA `lin` of the dK / dV part works on: those of the window first, key tiles slowest, heads and batch fastest.
 struct WindowPart {
     int j, b, g, h_first, heads;    // key tile, batch, kv head, query heads
-    int q_first, q_tiles;           // query tiles of each head (none or less: nothing to do, for the last far part of a late tile)
+    int q_first, q_tiles;           // query tiles of each head (none or less: nothing to do, for the last parts of a late tile)
     int slot;                       // of the scratch; -1: the CTA has the whole sum
     __host__ __device__ WindowPart(const AttnWindow& w, const AttnWindowParts& c, int B, int S, int nh, int nkv, int lin) {
         const int rep = nh / nkv, nq = (S + kAttnTile - 1) / kAttnTile, stride = nkv * c.head_parts * B;
         const bool far = lin >= c.near_ctas;
         const int rest = (far ? lin - c.near_ctas : lin) / stride, at = lin % stride, y = at % (nkv * c.head_parts);   // near_ctas is a multiple of stride
-        j = far ? rest / c.far_parts : rest;
+        const int parts = far ? c.far_parts : c.near_parts, tiles = far ? c.far_tiles : c.near_tiles;
+        j = rest / parts;
         b = at / (nkv * c.head_parts);
         g = y / c.head_parts;
         heads = rep / c.head_parts;
         h_first = g * rep + y % c.head_parts * heads;
-        const int near_end = window_last_query_tile(w, j, nq) + 1;
-        q_first = far ? near_end + rest % c.far_parts * c.far_tiles : j;
-        q_tiles = (far && q_first + c.far_tiles < nq ? q_first + c.far_tiles : far ? nq : near_end) - q_first;
-        slot = c.head_parts == 1 && (j >= c.sink_tiles || near_end >= nq) ? -1 : far ? c.near_slots + lin - c.near_ctas : lin;
+        const int near_end = window_last_query_tile(w, j, nq) + 1, end = far ? nq : near_end;
+        q_first = (far ? near_end : j) + (rest - j * parts) * tiles;
+        q_tiles = (q_first + tiles < end ? q_first + tiles : end) - q_first;
+        slot = c.head_parts * c.near_parts == 1 && (j >= c.sink_tiles || near_end >= nq) ? -1 : far ? c.near_slots + lin - c.near_ctas : lin;
     }
 };
 
@@ -933,7 +934,7 @@ attn_window_join_kernel(const AttnBwdParams p) {
     const int heads_all = p.nkv * p.B, j = lin / heads_all, g = lin % heads_all % p.nkv, b = lin % heads_all / p.nkv;
     const int nq = (p.S + kAttnTile - 1) / kAttnTile, near_last = window_last_query_tile(p.win, j, nq);
     const int far = j < p.cut.sink_tiles ? nq - 1 - near_last : 0;      // query tiles behind the window
-    if (p.cut.head_parts == 1 && far <= 0) return;
+    if (p.cut.head_parts * p.cut.near_parts == 1 && far <= 0) return;
     const int which = item >> 11, r = (item >> 4) & 127, c = (item & 15) * 2;
     if (j * kAttnTile + r >= p.S) return;
     const uint32_t at0 = which * 65536 + r * 512 + ((c ^ (r & 7)) << 4), at1 = which * 65536 + r * 512 + (((c + 1) ^ (r & 7)) << 4);
@@ -946,7 +947,8 @@ attn_window_join_kernel(const AttnBwdParams p) {
         s0.x += a.x; s0.y += a.y; s0.z += a.z; s0.w += a.w;
         s1.x += d.x; s1.y += d.y; s1.z += d.z; s1.w += d.w;
     };
-    for (int k = 0; k < p.cut.head_parts; ++k) add(static_cast<long long>(j) * stride + mine + k);
+    for (int n = 0; n < p.cut.near_parts && j + n * p.cut.near_tiles <= near_last; ++n)
+        for (int k = 0; k < p.cut.head_parts; ++k) add((static_cast<long long>(j) * p.cut.near_parts + n) * stride + mine + k);
     const int parts = far > 0 ? (far + p.cut.far_tiles - 1) / p.cut.far_tiles : 0;
     const long long far0 = p.cut.near_slots + static_cast<long long>(j) * p.cut.far_parts * stride + mine;
 #pragma unroll 4
@@ -958,8 +960,10 @@ attn_window_join_kernel(const AttnBwdParams p) {
         make_uint4(pack_bf16(s0.x * mul, s0.y * mul), pack_bf16(s0.z * mul, s0.w * mul), pack_bf16(s1.x * mul, s1.y * mul), pack_bf16(s1.z * mul, s1.w * mul));
 }
 
-// Whole numbers only, so that host and device agree on every size. Cutting is worth it where one CTA's steps would outlast everybody's share of all steps:
-// dK / dV of a step cost about 5 / 4 of dQ's.
+// Whole numbers only, so that host and device agree on every size. Cutting is worth it where one CTA's steps would outlast everybody's share of all steps
+// by more than the second kernel costs, which is that of three steps and a little for each part it reads: dK / dV of a step cost about 5 / 4 of dQ's. us of a
+// backward, whole tiles or cut by heads / by heads and query tiles: 4000 tokens, 1 head 63 / 51, 2 x 1500, 8 / 1 heads, window 100 38 / 35, 2000, 4 / 4 36 /
+// 33, 5 x 60, 24 / 3 22 / 18.
 AttnWindowParts window_parts(const AttnWindow& w, int B, int S, int nh, int nkv, int sms) {
     AttnWindowParts c = {};
     const int nq = (S + kAttnTile - 1) / kAttnTile, rep = nh / nkv;
@@ -970,12 +974,17 @@ AttnWindowParts window_parts(const AttnWindow& w, int B, int S, int nh, int nkv,
     long long steps = 0;     // of one head, in quarters of a dQ step
     for (int j = 0; j < nq; ++j) steps += 9ll * (j < c.sink_tiles ? nq - j : window_last_query_tile(w, j, nq) - j + 1);
     const long long share = steps * B * nh / sms;
-    c.head_parts = 1;
-    const long long join = 12;   // what the second kernel costs beyond its launch behind sink tiles, in the same unit
-    for (int k = 2; k <= rep; ++k)
-        if (rep % k == 0) {
-            const long long now = 5ll * near_most * (rep / c.head_parts), then = 5ll * near_most * (rep / k);
-            if ((now > share ? now : share) > (then > share ? then : share) + (c.head_parts == 1 && !c.sink_tiles ? join : 0)) c.head_parts = k;
+    long long best = -1;
+    for (int heads = 1; heads <= rep; ++heads)
+        for (int near = 1; rep % heads == 0 && near <= near_most; near *= 2) {
+            const int tiles = (near_most + near - 1) / near;
+            const long long longest = 5ll * tiles * (rep / heads), slots = groups * nq * heads * near;
+            const long long cost = (longest > share ? longest : share) + (heads * near > 1 ? (c.sink_tiles ? 0 : 12) + slots / 8 : 0);
+            if (best >= 0 && cost >= best) continue;
+            best = cost;
+            c.head_parts = heads;
+            c.near_tiles = tiles;
+            c.near_parts = (near_most + tiles - 1) / tiles;
         }
     const long long heads_all = groups * c.head_parts;
     if (c.sink_tiles) {
@@ -985,9 +994,9 @@ AttnWindowParts window_parts(const AttnWindow& w, int B, int S, int nh, int nkv,
         c.far_tiles = static_cast<int>(tiles < far_most ? tiles : far_most);
         c.far_parts = (far_most + c.far_tiles - 1) / c.far_tiles;
     }
-    c.near_ctas = static_cast<int>(nq * heads_all);
+    c.near_ctas = static_cast<int>(nq * heads_all * c.near_parts);
     c.far_ctas = static_cast<int>(c.sink_tiles * heads_all * c.far_parts);
-    c.near_slots = static_cast<int>(c.head_parts > 1 ? c.near_ctas : c.sink_tiles * heads_all);
+    c.near_slots = static_cast<int>(c.head_parts * c.near_parts > 1 ? c.near_ctas : c.sink_tiles * heads_all);
     return c;
 }
 
@@ -1089,7 +1098,10 @@ CAI_API int cai_flash_attn_window_walk(int B, int S, int nh, int nkv, int window
 }
 CAI_API int cai_flash_attn_window_keys(int S, int window, int sinks, int i, int* tiles, int capacity) {
     const WindowKeys keys({window < S ? window : S, sinks < S ? sinks : S}, i);
-    for (int k = 0; k < keys.n && k < capacity; ++k) tiles[k] = keys.tile(k);
+    for (int k = 0; k < keys.n && k < capacity; ++k) {
+        tiles[2 * k] = keys.tile(k);
+        tiles[2 * k + 1] = keys.width({window < S ? window : S, sinks < S ? sinks : S}, k);
+    }
     return keys.n;
 }
 
@@ -1145,7 +1157,7 @@ CAI_API int cai_flash_attn_window_bwd(const void* qkv, long long ld, const void*
     if (e == cudaSuccess)
         e = launch_early(attn_bwd_kernel<true>, static_cast<unsigned>(kv_ctas + q_ctas), kAttnBwdThreads, kAttnBwdSmem, st, tm_qkv, tm_do, p, kv_ctas);
     if (e == cudaSuccess && p.cut.near_slots + p.cut.far_ctas > 0) {
-        const long long tiles = p.cut.head_parts > 1 ? (S + kAttnTile - 1) / kAttnTile : p.cut.sink_tiles;
+        const long long tiles = p.cut.head_parts * p.cut.near_parts > 1 ? (S + kAttnTile - 1) / kAttnTile : p.cut.sink_tiles;
         e = launch_early(attn_window_join_kernel, static_cast<unsigned>(tiles * nkv * B * 16), 256, 0, st, p);
     }
     if (e != cudaSuccess) {

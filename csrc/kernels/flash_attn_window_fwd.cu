@@ -24,8 +24,8 @@ struct Divisor {
     uint32_t m;
     Divisor() = default;
     explicit Divisor(int by) : d(by), m(by == 1 ? 0xffffffffu : static_cast<uint32_t>((1ull << 32) / static_cast<uint32_t>(by))) {}
-    __device__ __forceinline__ int quotient(int n) const {
-        const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(n), m));
+    __host__ __device__ __forceinline__ int quotient(int n) const {
+        const int q = static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * m) >> 32);
         return q + (n - q * d >= d);
     }
 };
@@ -92,9 +92,23 @@ struct WindowBlocks {
     __host__ __device__ int block(int j) const { return j < sinks ? j : lo + j - sinks; }
 };
 
-// The blocks of keys that a CTA takes, item after item. Rounds of items go to and fro, so that nobody gets the longest of each.
-struct WindowStream {
-    int round, tile, h, b;
+// Item number `round` of CTA `cta` of `ctas`: rounds go to and fro, so that nobody gets the longest item of each.
+__host__ __device__ __forceinline__ int item_of(int round, int cta, int ctas) { return round * ctas + ((round & 1) ? ctas - 1 - cta : cta); }
+// An item: latest query tiles, which have the most keys, of every head first.
+struct WindowTile {
+    int tile, h, b;
+    WindowTile() = default;
+    __host__ __device__ __forceinline__ WindowTile(int item, int tiles, const Divisor& heads_all, const Divisor& heads) {
+        const int row = heads_all.quotient(item), at = item - row * heads_all.d;
+        tile = tiles - 1 - row;
+        b = heads.quotient(at);
+        h = at - b * heads.d;
+    }
+};
+
+// The blocks of keys that a CTA takes, item after item.
+struct WindowStream : WindowTile {
+    int round;
     int u;                 // block of the item
     WindowBlocks keys;
     __device__ WindowStream(const WindowFwdParams& p) : round(-1), u(0) { keys.n = 0; next_item(p); }
@@ -104,14 +118,11 @@ struct WindowStream {
     __device__ int row() const { return keys.block(u) * kBlock; }
     __device__ void next_item(const WindowFwdParams& p) {
         ++round;
-        const int item = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        const int item = item_of(round, blockIdx.x, gridDim.x);
         u = 0;
         keys.n = 0;
         if (item >= p.items) return;     // of the last round, which nothing follows
-        const int row = p.heads_all.quotient(item), at = item - row * p.heads_all.d;
-        tile = p.tiles - 1 - row;   // latest query tiles, which have the most keys, of every head first
-        b = p.heads.quotient(at);
-        h = at - b * p.nh;
+        static_cast<WindowTile&>(*this) = WindowTile(item, p.tiles, p.heads_all, p.heads);
         keys = WindowBlocks(p.win, tile, p.S);
     }
     __device__ void next(const WindowFwdParams& p) {
@@ -130,7 +141,7 @@ struct WindowCount {
     __device__ int width(const WindowFwdParams& p, int u) const { return u < sinks ? seen_sinks(p.win, u * kBlock, kBlock) : kBlock; }
     __device__ void next_item(const WindowFwdParams& p) {
         ++round;
-        const int item = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        const int item = item_of(round, blockIdx.x, gridDim.x);
         left = n = 0;
         if (item >= p.items) return;
         const WindowBlocks blocks(p.win, p.tiles - 1 - p.heads_all.quotient(item), p.S);
@@ -440,6 +451,32 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tm, const WindowFwdPa
 }  // namespace cai
 
 using namespace cai;
+
+CAI_API int cai_flash_attn_window_blocks(int S, int window, int sinks, int i, int* blocks, int capacity) {
+    const AttnWindow w = {window < S ? window : S, sinks < S ? sinks : S};
+    const WindowBlocks b(w, i, S);
+    for (int k = 0; k < b.n && k < capacity; ++k) {
+        blocks[2 * k] = b.block(k);
+        blocks[2 * k + 1] = k < b.sinks ? seen_sinks(w, k * kBlock, kBlock) : kBlock;
+    }
+    return b.n;
+}
+CAI_API int cai_flash_attn_window_items(int B, int S, int nh, int ctas, int cta, int* items, int capacity) {
+    const int tiles = (S + kAttnTile - 1) / kAttnTile, all = tiles * nh * B;
+    const Divisor heads_all(nh * B), heads(nh);
+    int n = 0;
+    for (int round = 0;; ++round) {
+        const int item = item_of(round, cta, ctas);
+        if (item >= all) return n;
+        if (n < capacity) {
+            const WindowTile t(item, tiles, heads_all, heads);
+            items[3 * n] = t.tile;
+            items[3 * n + 1] = t.h;
+            items[3 * n + 2] = t.b;
+        }
+        ++n;
+    }
+}
 
 CAI_API int cai_flash_attn_window_fwd(const void* qkv, long long ld, void* out, float* lse, int B, int S, int nh, int nkv, int hd, float scale,
                                       int window, int sinks, void* stream) {

@@ -32,18 +32,58 @@ SHAPES = [(1, 1, 1, 1, 1, 0), (2, 128, 2, 1, 64, 4), (3, 129, 4, 2, 1, 0), (1, 1
           (1, 16384, 2, 1, 300, 1), (1, 3000, 16, 2, 127, 300)]
 
 
+def _taken(call, S, window, sinks, i):
+    """(number, keys that the products take) of what query tile i takes."""
+    found = (ctypes.c_int * 8192)()
+    n = call(S, window, sinks, i, found, 4096)
+    assert 0 < n <= 4096
+    return [(found[2 * k], found[2 * k + 1]) for k in range(n)]
+
+
 @pytest.mark.parametrize("B,S,nh,nkv,window,sinks", SHAPES)
-def test_forward_takes_every_key_tile_once(B, S, nh, nkv, window, sinks):
+def test_dq_takes_every_key_tile_once(B, S, nh, nkv, window, sinks):
     from cai_b200.ops import lib
-    want = _tile_pairs(S, window, sinks)
-    got = []
+    got = set()
     for i in range((S + T - 1) // T):
-        tiles = (ctypes.c_int * 4096)()
-        n = lib().cai_flash_attn_window_keys(S, window, sinks, i, tiles, 4096)
-        assert 0 < n <= 4096 and list(tiles[:n]) == sorted(tiles[:n]) and tiles[n - 1] == i, "in order, the diagonal last"
-        got += [(i, tiles[k]) for k in range(n)]
-    assert len(got) == len(set(got))
-    assert set(got) == want
+        tiles = _taken(lib().cai_flash_attn_window_keys, S, window, sinks, i)
+        numbers = [t for t, _ in tiles]
+        assert numbers == sorted(set(numbers)) and numbers[-1] == i, "in order, the diagonal last"
+        for t, width in tiles:
+            # all keys, or of a tile that is behind every window of the query tile the sinks, 16 at a time
+            assert width == T or (width % 16 == 0 and sinks <= t * T + width < sinks + 16 and (t + 1) * T - 1 <= i * T - window)
+        got |= {(i, t) for t in numbers}
+    assert got == _tile_pairs(S, window, sinks)
+
+
+@pytest.mark.parametrize("B,S,nh,nkv,window,sinks", SHAPES)
+def test_forward_takes_every_block_of_keys_once(B, S, nh, nkv, window, sinks):
+    from cai_b200.ops import lib
+    K = 64
+    for i in range((S + T - 1) // T):
+        blocks = _taken(lib().cai_flash_attn_window_blocks, S, window, sinks, i)
+        numbers = [k for k, _ in blocks]
+        assert numbers == sorted(set(numbers))
+        q_first, q_last = i * T, min(S, (i + 1) * T) - 1
+        want = [k for k in range(q_last // K + 1) if min(k * K + K - 1, q_first) > q_first - window or k * K < sinks]
+        assert numbers == want
+        for k, width in blocks:
+            assert width == K or (width % 16 == 0 and sinks <= k * K + width < sinks + 16 and (k + 1) * K - 1 <= q_first - window)
+
+
+@pytest.mark.parametrize("B,S,nh,ctas", [(1, 1, 1, 1), (3, 300, 5, 45), (4, 4096, 16, 296), (1, 2000, 32, 296), (2, 9000, 3, 296), (7, 130, 9, 17), (1, 32768, 4, 296)])
+def test_forward_items_are_taken_once(B, S, nh, ctas):
+    from cai_b200.ops import lib
+    seen, most, least = set(), 0, 1 << 30
+    for cta in range(ctas):
+        found = (ctypes.c_int * 30000)()
+        n = lib().cai_flash_attn_window_items(B, S, nh, ctas, cta, found, 10000)
+        most, least = max(most, n), min(least, n)
+        for k in range(n):
+            t = tuple(found[3 * k:3 * k + 3])
+            assert t not in seen
+            seen.add(t)
+    assert seen == {(i, h, b) for i in range((S + T - 1) // T) for h in range(nh) for b in range(B)}
+    assert most - least <= 1
 
 
 @pytest.mark.parametrize("sms", [148, 8, 1])
