@@ -345,8 +345,8 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tm, const WindowFwdPa
         int c = 0;       // block of the stream
         for (WindowStream at(p); at.there() && ok; at.next_item(p)) {
             const int q0 = at.tile * kAttnTile;
-            // A window may hide a whole row of a block, so that its maximum starts at a finite number: exp2(-inf - m) is 0 then as well.
-            float m_used = -1e30f;
+            // A window may hide a whole row of a block, so that its maximum starts at the lowest finite number: exp2(-inf - m) is 0 then as well.
+            float m_used = -3.4028234664e38f;
             uint64_t l2 = 0;
 #pragma unroll 1
             for (int u = 0; u < at.keys.n; ++u, ++c) {

@@ -180,6 +180,15 @@ int64_t packed_pitch(const char* op, const at::Tensor& t, int64_t rows, int64_t 
     need((cols < 2 || t.stride(1) == 1) && (rows < 2 || t.stride(0) >= cols), op, "rows have to be contiguous and apart");
     return rows > 1 ? t.stride(0) : cols;
 }
+// Do two packed tensors share memory? (Columns of one buffer beside each other do not.)
+bool overlap(const at::Tensor& a, int64_t lda, const at::Tensor& b, int64_t ldb) {
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    const auto at = reinterpret_cast<uintptr_t>(a.data_ptr()) / 2, bt = reinterpret_cast<uintptr_t>(b.data_ptr()) / 2;     // in elements
+    if (at + (a.size(0) - 1) * lda + a.size(1) <= bt || bt + (b.size(0) - 1) * ldb + b.size(1) <= at) return false;
+    if (lda != ldb) return true;
+    const int64_t off = ((static_cast<int64_t>(bt) - static_cast<int64_t>(at)) % lda + lda) % lda;     // b's first column, from a's
+    return off < a.size(1) || off + b.size(1) > lda;
+}
 struct WindowCall {
     int B, S, nh, nkv, hd, window, sinks;
     float scale;
@@ -220,8 +229,11 @@ PyObject* window_bwd(PyObject* const* a) {
     const at::Tensor *dqkv = tensor_or_none(a[12], op), *delta = tensor_or_none(a[13], op), *scratch = tensor_or_none(a[14], op);
     const int64_t ld = packed_pitch(op, qkv, c.rows, c.cols), ldq = dqkv ? packed_pitch(op, *dqkv, c.rows, c.cols) : c.cols;
     const int64_t width = static_cast<int64_t>(c.nh) * c.hd, stats = c.rows * c.nh;
-    for (const at::Tensor* t : {&out, &dout})
+    for (const at::Tensor* t : {&out, &dout}) {
         need(t->scalar_type() == at::kBFloat16 && shaped(*t, c.rows, width) && t->is_contiguous(), op, "out and dout are bf16 [B * S, heads * head_dim]");
+        need(!dqkv || !overlap(*t, width, *dqkv, ldq), op, "dqkv shares memory with what is read");
+    }
+    need(!dqkv || !overlap(qkv, ld, *dqkv, ldq), op, "dqkv shares memory with what is read");
     need(lse.scalar_type() == at::kFloat && lse.dim() == 3 && lse.size(0) == c.B && lse.size(1) == c.nh && lse.size(2) == c.S && lse.is_contiguous(), op,
          "lse is f32 [B, heads, S]");
     if (delta) need(delta->scalar_type() == at::kFloat && delta->numel() >= stats && delta->is_contiguous(), op, "delta is f32 [B, heads, S]");

@@ -273,6 +273,25 @@ def test_captured_and_replayed():
             assert torch.equal(x, y)
 
 
+def test_gradients_over_what_is_read_are_refused():
+    """dqkv in qkv's, out's or dout's place; beside qkv in one buffer it is taken."""
+    from cai_b200 import ops
+    S, nh, nkv, cols = 150, 2, 1, 4 * HD
+    both = torch.randn(S, 2 * cols, device="cuda").to(torch.bfloat16)
+    qkv, dqkv = both[:, :cols], both[:, cols:]
+    dout = torch.randn(S, nh * HD, device="cuda").to(torch.bfloat16)
+    out, lse = ops.flash_attn_window_fwd(qkv, 1, S, nh, nkv, HD, 20)
+    want = ops.flash_attn_window_bwd(qkv, out, dout, lse, 1, S, nh, nkv, HD, 20)
+    for bad in (qkv, both[:, HD:HD + cols], both[:, cols - 8:2 * cols - 8]):
+        with pytest.raises(ops.KernelError, match="shares memory"):
+            ops.flash_attn_window_bwd(qkv, out, dout, lse, 1, S, nh, nkv, HD, 20, dqkv=bad)
+    wide = torch.empty(S * cols, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ops.KernelError, match="shares memory"):
+        ops.flash_attn_window_bwd(qkv, out, wide[:S * nh * HD].view(S, nh * HD), lse, 1, S, nh, nkv, HD, 20, dqkv=wide.view(S, cols))
+    assert ops.flash_attn_window_bwd(qkv, out, dout, lse, 1, S, nh, nkv, HD, 20, dqkv=dqkv) is dqkv
+    assert torch.equal(dqkv, want)
+
+
 def test_no_rows():
     from cai_b200 import ops
     for B, S in ((0, 5), (3, 0)):
