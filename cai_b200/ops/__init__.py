@@ -289,13 +289,15 @@ def flash_attn_window_fwd(qkv, B, S, nh, nkv, hd, window, sinks=0, scale=None):
 def flash_attn_window_bwd(qkv, out, dout, lse, B, S, nh, nkv, hd, window, sinks=0, scale=None, dqkv=None, delta=None, scratch=None):
     """Gradient of :func:`flash_attn_window_fwd` with respect to ``qkv``, packed like it (``dqkv``, made where it is None). ``out`` and ``lse`` are the forward
     pass's, ``dout`` the gradient of ``out``. ``delta`` (f32 ``[B, nh, S]``) and ``scratch`` (uint8, :func:`flash_attn_window_bwd_scratch` bytes) are
-    workspaces, made where they are None; calls that may overlap need their own. The same bits in every run."""
+    workspaces, made where they are None; they share no memory with another argument, and calls that may overlap need their own. The same bits in every
+    run."""
     return native().flash_attn_window_bwd(qkv, out, dout, lse, B, S, nh, nkv, hd, window, sinks, scale, dqkv, delta, scratch)
 
 
 def flash_attn_window_bwd_scratch(B, S, nh, nkv, window, sinks=0):
     """Bytes of scratch :func:`flash_attn_window_bwd` takes on the current device."""
-    return calls().cai_flash_attn_window_bwd_scratch(B, S, nh, nkv, window, sinks)
+    most = 2 ** 31 - 1     # no sequence is longer
+    return calls().cai_flash_attn_window_bwd_scratch(B, S, nh, nkv, min(window, most), min(sinks, most))
 
 
 __all__ = [n for n in dir() if not n.startswith("_")]

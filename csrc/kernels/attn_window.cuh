@@ -48,13 +48,5 @@ __device__ __forceinline__ void load_seq_tile(void* dst, const CUtensorMap* tm, 
     tma_load_3d(dst, tm, bar, x, row, b);
     tma_load_3d(static_cast<uint8_t*>(dst) + kAttnSub, tm, bar, x + 64, row, b);
 }
-// Half `half` of the keys of O[128,hd] (+)= P[128,128](TMEM, bf16 pairs) * V[128,hd].
-__device__ __forceinline__ void issue_pv_half(uint32_t d_tmem, uint32_t p_tmem, uint64_t v_desc, uint32_t idesc, int half, bool accumulate) {
-#pragma unroll
-    for (int k = 0; k < kAttnTile / 32; ++k) {
-        const int i = half * (kAttnTile / 32) + k;
-        umma_f16_ts(d_tmem, p_tmem + i * 8, v_desc + i * (2048 >> 4), idesc, (accumulate || k > 0) ? 1u : 0u);
-    }
-}
 
 }  // namespace cai

@@ -189,6 +189,16 @@ bool overlap(const at::Tensor& a, int64_t lda, const at::Tensor& b, int64_t ldb)
     const int64_t off = ((static_cast<int64_t>(bt) - static_cast<int64_t>(at)) % lda + lda) % lda;     // b's first column, from a's
     return off < a.size(1) || off + b.size(1) > lda;
 }
+// Workspaces are written while everything else is in use.
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+    const auto end = [](const at::Tensor& t) {
+        int64_t last = 0;
+        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+        return reinterpret_cast<uintptr_t>(t.data_ptr()) + (last + 1) * t.element_size();
+    };
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    return reinterpret_cast<uintptr_t>(a.data_ptr()) < end(b) && reinterpret_cast<uintptr_t>(b.data_ptr()) < end(a);
+}
 struct WindowCall {
     int B, S, nh, nkv, hd, window, sinks;
     float scale;
@@ -236,7 +246,11 @@ PyObject* window_bwd(PyObject* const* a) {
     need(!dqkv || !overlap(qkv, ld, *dqkv, ldq), op, "dqkv shares memory with what is read");
     need(lse.scalar_type() == at::kFloat && lse.dim() == 3 && lse.size(0) == c.B && lse.size(1) == c.nh && lse.size(2) == c.S && lse.is_contiguous(), op,
          "lse is f32 [B, heads, S]");
+    need(!dqkv || !overlap(lse, *dqkv), op, "dqkv shares memory with what is read");
     if (delta) need(delta->scalar_type() == at::kFloat && delta->numel() >= stats && delta->is_contiguous(), op, "delta is f32 [B, heads, S]");
+    for (const at::Tensor* w : {delta, scratch})
+        for (const at::Tensor* t : {&qkv, &out, &dout, &lse, dqkv, w == scratch ? delta : nullptr})
+            need(!w || !t || !overlap(*w, *t), op, "a workspace shares memory with another argument");
     const Place at = place(op, {&qkv, &out, &dout, &lse, dqkv, delta, scratch});
     const int64_t bytes = cai_flash_attn_window_bwd_scratch(c.B, c.S, c.nh, c.nkv, c.window, c.sinks);
     if (scratch) need(static_cast<int64_t>(scratch->nbytes()) >= bytes && scratch->is_contiguous(), op, "the scratch is too small, see flash_attn_window_bwd_scratch");

@@ -186,6 +186,41 @@ def test_window_calls_refuse_tensors_that_do_not_fit():
             ops.flash_attn_window_bwd(qkv, o, d, l, B, S, nh, nkv, 128, 4)
 
 
+def test_window_bwd_refuses_workspaces_and_gradients_over_other_arguments():
+    """lse's place for delta would give no error and wrong gradients: every CTA reads lse while delta is written."""
+    from cai_b200 import ops
+    B, S, nh, nkv = 2, 300, 2, 1
+    bf16, n = torch.bfloat16, 600
+    qkv, out, dout, lse = torch.zeros(n, 512, dtype=bf16), torch.zeros(n, 256, dtype=bf16), torch.zeros(n, 256, dtype=bf16), torch.zeros(B, nh, S)
+    dqkv, delta = torch.zeros(n, 512, dtype=bf16), torch.zeros(B, nh, S)
+    need = ops.flash_attn_window_bwd_scratch(B, S, nh, nkv, 40, 3)
+    assert need > 0
+    both = torch.zeros(need + 4 * B * nh * S, dtype=torch.uint8)
+
+    def of(t, dtype=torch.float32):
+        return t.view(-1).view(dtype)
+    cases = [dict(delta=lse), dict(delta=of(qkv)), dict(delta=of(out)), dict(delta=of(dout)[-B * nh * S:]), dict(dqkv=dqkv, delta=of(dqkv)),
+             dict(scratch=both[4 * B * nh * S - 16:], delta=both[:4 * B * nh * S].view(torch.float32))]
+    for change in cases:
+        with pytest.raises(ops.KernelError, match="flash_attn_window_bwd: a workspace shares memory"):
+            ops.flash_attn_window_bwd(qkv, out, dout, lse, B, S, nh, nkv, 128, 40, 3, **change)
+    wide = torch.zeros(n * 512, dtype=bf16)
+    with pytest.raises(ops.KernelError, match="flash_attn_window_bwd: dqkv shares memory"):
+        ops.flash_attn_window_bwd(qkv, out, dout, of(wide)[:B * nh * S].view(B, nh, S), B, S, nh, nkv, 128, 40, 3, dqkv=wide.view(n, 512))
+    # beside one another they are taken: what is refused is the device
+    for change in (dict(delta=delta, dqkv=dqkv), dict(scratch=both[4 * B * nh * S:], delta=both[:4 * B * nh * S].view(torch.float32))):
+        with pytest.raises(ops.KernelError, match="current device"):
+            ops.flash_attn_window_bwd(qkv, out, dout, lse, B, S, nh, nkv, 128, 40, 3, **change)
+
+
+def test_scratch_of_a_window_wider_than_any_sequence():
+    from cai_b200 import ops
+    want = ops.flash_attn_window_bwd_scratch(1, 4000, 1, 1, 4000, 4000)
+    assert want > 0
+    for window, sinks in ((2 ** 31, 0), (2 ** 32, 2 ** 32 + 1), (2 ** 40, 2 ** 62)):
+        assert ops.flash_attn_window_bwd_scratch(1, 4000, 1, 1, window, sinks) == want
+
+
 def _rope(**change):
     a = dict(qkv=P, freqs=P, pos=P, ldp=10, T=10, nh=2, nkv=1, hd=128, ld=512, axes=3, n0=16, n1=24, n2=24, n3=0, interleaved=0, inverse=0, stream=0)
     a.update(change)
