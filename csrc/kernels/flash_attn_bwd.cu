@@ -616,7 +616,13 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
             if (part.slot >= 0) {
                 if (ok && threadIdx.x == 128) {
                     char* to = reinterpret_cast<char*>(p.partial) + part.slot * 131072ll;
-                    for (int k = 0; k < 8; ++k) bulk_store(to + k * 16384, smem + k * 16384, 16384);
+                    if (lin < p.cut.near_ctas) {
+                        for (int k = 0; k < 8; ++k) bulk_store(to + k * 16384, smem + k * 16384, 16384);
+                    } else {      // behind the window only the sinks' rows are other than zero
+                        const int bytes = seen_sinks(p.win, j * kAttnTile, kAttnTile) * 512;
+                        bulk_store(to, smem, bytes);
+                        bulk_store(to + 65536, smem + 65536, bytes);
+                    }
                     tma_store_commit();
                     tma_store_wait0();
                 }
@@ -949,7 +955,7 @@ attn_window_join_kernel(const AttnBwdParams p) {
     };
     for (int n = 0; n < p.cut.near_parts && j + n * p.cut.near_tiles <= near_last; ++n)
         for (int k = 0; k < p.cut.head_parts; ++k) add((static_cast<long long>(j) * p.cut.near_parts + n) * stride + mine + k);
-    const int parts = far > 0 ? (far + p.cut.far_tiles - 1) / p.cut.far_tiles : 0;
+    const int parts = far > 0 && j * kAttnTile + r < p.win.sinks ? (far + p.cut.far_tiles - 1) / p.cut.far_tiles : 0;
     const long long far0 = p.cut.near_slots + static_cast<long long>(j) * p.cut.far_parts * stride + mine;
 #pragma unroll 4
     for (int f = 0; f < parts; ++f)
