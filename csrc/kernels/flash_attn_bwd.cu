@@ -532,11 +532,18 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
                 const int from = (j - i) * kAttnTile + r - qb;
                 seen = ~bits_below(from) & (j * kAttnTile + r < p.win.sinks ? ~0u : bits_below(from + p.win.window));
             }
+            // Of a tile at either end of the window six of sixteen warps see nothing, of a sinks' tile behind it at least twelve: zeros, for no exponentials.
+            const bool none = kWindow && diag && !__any_sync(0xffffffffu, seen);
             const float delta = delta_next;
             if (!mbar_wait_warp(s_full, it & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
             tc_fence_after();
             uint32_t pr[32];
-            tmem_ld_32x32(tSg, pr);
+            if (none) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) pr[e] = 0;
+            } else {
+                tmem_ld_32x32(tSg, pr);
+            }
             __syncwarp();
             stat[lane] = lse_next * (kWindow ? -1.4426950408889634f : 1.4426950408889634f);
             if (it + 1 < iters) {
@@ -550,12 +557,12 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
             tmem_ld_wait();
             tc_fence_before();
             mbar_arrive_warp(s_empty);
-            if constexpr (kWindow) window_prob_cols<0>(pr, ls, p.scale_log2, diag, seen);
+            if constexpr (kWindow) { if (!none) window_prob_cols<0>(pr, ls, p.scale_log2, diag, seen); }
             else if (diag) prob_cols<true, 0>(pr, ls, p.scale_log2, r, qb);
             else prob_cols<false, 0>(pr, ls, p.scale_log2, r, qb);
 #pragma unroll
             for (int e = 0; e < 4; ++e) ls[e] = reinterpret_cast<const float4*>(stat)[4 + e];
-            if constexpr (kWindow) window_prob_cols<1>(pr, ls, p.scale_log2, diag, seen);
+            if constexpr (kWindow) { if (!none) window_prob_cols<1>(pr, ls, p.scale_log2, diag, seen); }
             else if (diag) prob_cols<true, 1>(pr, ls, p.scale_log2, r, qb);
             else prob_cols<false, 1>(pr, ls, p.scale_log2, r, qb);
             __syncwarp();
@@ -577,22 +584,27 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
             if (!mbar_wait_warp(dp_full, it & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
             tc_fence_after();
             uint32_t dp[32];
-            tmem_ld_32x32(tdPg, dp);
-            tmem_ld_wait();
             uint32_t dk[16];
+            if (none) {
 #pragma unroll
-            for (int e4 = 0; e4 < 8; ++e4) {
-                const float4 d = reinterpret_cast<const float4*>(stat)[e4];
-                const int e = e4 * 4;
-                if constexpr (kWindow) {
-                    dk[e4 * 2] = window_ds(pr[e], pr[e + 1], dp[e], dp[e + 1], d.x, d.y);
-                    dk[e4 * 2 + 1] = window_ds(pr[e + 2], pr[e + 3], dp[e + 2], dp[e + 3], d.z, d.w);
-                    continue;
+                for (int e = 0; e < 16; ++e) dk[e] = 0;
+            } else {
+                tmem_ld_32x32(tdPg, dp);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e4 = 0; e4 < 8; ++e4) {
+                    const float4 d = reinterpret_cast<const float4*>(stat)[e4];
+                    const int e = e4 * 4;
+                    if constexpr (kWindow) {
+                        dk[e4 * 2] = window_ds(pr[e], pr[e + 1], dp[e], dp[e + 1], d.x, d.y);
+                        dk[e4 * 2 + 1] = window_ds(pr[e + 2], pr[e + 3], dp[e + 2], dp[e + 3], d.z, d.w);
+                        continue;
+                    }
+                    dk[e4 * 2] = pack_bf16(__uint_as_float(pr[e]) * (__uint_as_float(dp[e]) - d.x),
+                                           __uint_as_float(pr[e + 1]) * (__uint_as_float(dp[e + 1]) - d.y));
+                    dk[e4 * 2 + 1] = pack_bf16(__uint_as_float(pr[e + 2]) * (__uint_as_float(dp[e + 2]) - d.z),
+                                               __uint_as_float(pr[e + 3]) * (__uint_as_float(dp[e + 3]) - d.w));
                 }
-                dk[e4 * 2] = pack_bf16(__uint_as_float(pr[e]) * (__uint_as_float(dp[e]) - d.x),
-                                       __uint_as_float(pr[e + 1]) * (__uint_as_float(dp[e + 1]) - d.y));
-                dk[e4 * 2 + 1] = pack_bf16(__uint_as_float(pr[e + 2]) * (__uint_as_float(dp[e + 2]) - d.z),
-                                           __uint_as_float(pr[e + 3]) * (__uint_as_float(dp[e + 3]) - d.w));
             }
             tmem_st_32x16(tdPg, dk);
             tmem_st_wait();
@@ -831,23 +843,37 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
 #pragma unroll 1
         for (int j = 0; j < n; ++j) {
             const int buf = j & 1;
+            // kWindow: the 32 columns this thread's query sees, a bit each: up to its own key, of the window or the sinks. (Past a sinks' tile's width the columns hold
+            // anything; they are not seen, and dQ does not read what becomes of them.)
+            const int kt = kWindow ? keys.tile(j) : j;
+            const bool hides = kWindow && window_masks(p.win, i, kt);
+            uint32_t seen = ~0u;
+            if (hides) {
+                const int last = (i - kt) * kAttnTile + r - kb;
+                seen = bits_below(last + 1) & (~bits_below(last + 1 - p.win.window) | bits_below(p.win.sinks - kt * kAttnTile - kb));
+            }
+            const bool none = hides && !__any_sync(0xffffffffu, seen);
             if (!mbar_wait_warp(&s_full[buf], (j >> 1) & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
             tc_fence_after();
+            if (none) {
+                mbar_arrive_warp(&s_empty[buf]);
+                if (!mbar_wait_warp(dp_full, j & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
+                tc_fence_after();
+                uint32_t zero[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) zero[e] = 0;
+                tmem_st_32x16(tdPg, zero);
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive_warp(ds_ready);
+                continue;
+            }
             uint32_t pr[32];
             tmem_ld_32x32(tS + buf * 128 + lane_bits + kb, pr);
             tmem_ld_wait();
             tc_fence_before();
             mbar_arrive_warp(&s_empty[buf]);
             if constexpr (kWindow) {
-                // the 32 columns this thread's query sees, a bit each: up to its own key, of the window or the sinks. (Past a sinks' tile's width the columns hold
-                // anything; they are not seen, and dQ does not read what becomes of them.)
-                const int kt = keys.tile(j);
-                const bool hides = window_masks(p.win, i, kt);
-                uint32_t seen = ~0u;
-                if (hides) {
-                    const int last = (i - kt) * kAttnTile + r - kb;
-                    seen = bits_below(last + 1) & (~bits_below(last + 1 - p.win.window) | bits_below(p.win.sinks - kt * kAttnTile - kb));
-                }
                 window_prob_rows(pr, -lse2, p.scale_log2, hides, seen);
             } else {
                 if (j == i) prob_rows<true>(pr, lse2, p.scale_log2, r, kb);
