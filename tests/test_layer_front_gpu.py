@@ -57,6 +57,28 @@ def test_norm_of_many_rows():
     _check_norm(x, r, g, 1e-6, ops.add_rmsnorm_quant(x, r, g, keep_y=True))
 
 
+@pytest.mark.parametrize("rows,H", [(1, 128), (5, 384), (333, 1408)])
+def test_norm_results_are_apart(rows, H):
+    """Results share allocations: each starts on 16 bytes, ends before the next one, and is changed without the others; one that is kept keeps its values."""
+    from cai_b200 import ops
+    x, r, g = _norm_inputs(rows, H, 6)
+    got = ops.add_rmsnorm_quant(x, r, g, keep_y=True)
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in got)
+    assert all(a % 16 == 0 for a, _ in spans[:1]) and all(t.data_ptr() % 16 == 0 for t in got[:3])
+    assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+    for t in got:
+        assert t.is_contiguous() and t.data_ptr() + t.numel() * t.element_size() <= t.untyped_storage().data_ptr() + t.untyped_storage().nbytes()
+    want = [t.clone() for t in got]
+    for i, t in enumerate(got):
+        t.view(torch.uint8).fill_(0x3c)
+        for k in range(i + 1, len(got)):
+            assert torch.equal(got[k].view(torch.uint8), want[k].view(torch.uint8))
+    h, q, s, rstd, y = ops.add_rmsnorm_quant(x, r, g, keep_y=True)
+    del h, y, q
+    other = [torch.full((rows, H), 7.0, device="cuda", dtype=torch.bfloat16) for _ in range(8)]
+    assert torch.equal(s, want[2]) and torch.equal(rstd, want[3]) and len(other) == 8
+
+
 def test_norm_of_views():
     """Rows with pitches of their own, a residual that is one row for all, rows that start in the middle of a buffer of NaN."""
     from cai_b200 import ops
