@@ -180,10 +180,8 @@ __device__ __forceinline__ void stage_acc_chunk(uint32_t tacc, uint32_t stage, i
 // A thread of 512 takes kPieces times eight columns and the eight that are 64 further on: item `first` of eight a row, 128 rows a tile of 64 KB, then
 // every 512th. Tile t leaves at dst[t], times mul[t]; where `rope` is given (the row of its table that belongs to row 0), tile 0 is rounded, as it
 // would be in memory, and rotated back.
-// kCut: only the tiles' first `rows` rows are there.
-template <bool kAdd, int kPieces, bool kCut = false>
-__device__ __forceinline__ void write_staged(uint32_t stage, __nv_bfloat16* const (&dst)[2], const float (&mul)[2], long long ld, int first, const float2* rope,
-                                             int rows = kAttnTile) {
+template <bool kAdd, int kPieces>
+__device__ __forceinline__ void write_staged(uint32_t stage, __nv_bfloat16* const (&dst)[2], const float (&mul)[2], long long ld, int first, const float2* rope) {
     uint4 old[kPieces][2];
     if constexpr (kAdd) {
 #pragma unroll
@@ -198,7 +196,6 @@ __device__ __forceinline__ void write_staged(uint32_t stage, __nv_bfloat16* cons
     for (int i = 0; i < kPieces; ++i) {
         const int item = first + i * 512, r = (item >> 3) & 127, c = (item & 7) * 2;
         const uint32_t row = stage + (i >> 1) * 65536 + r * 512;
-        if (kCut && r >= rows) continue;
         uint32_t o[2][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -234,6 +231,34 @@ __device__ __forceinline__ void write_staged(uint32_t stage, __nv_bfloat16* cons
 #pragma unroll
         for (int h = 0; h < 2; ++h)
             *reinterpret_cast<uint4*>(dst[i >> 1] + r * ld + h * 64 + (item & 7) * 8) = make_uint4(o[h][0], o[h][1], o[h][2], o[h][3]);
+    }
+}
+
+// A part's sums in the scratch: four columns (of piece c of 32) of row r of dK or dV at this float, eight rows to a line of 128 bytes.
+__device__ __forceinline__ int window_part_at(int which, int r, int c) { return which * 16384 + ((r >> 3) * 32 + c) * 32 + (r & 7) * 4; }
+
+// The windowed form, which adds to nothing and turns nothing, leaves by TMA in bf16: 32 columns of a thread's row, times `mul`, to chunk `chunk` on of its row in a
+// sub-tile of 64. (us, through write_staged / so: 2 x 128 tokens, 2 / 1 heads 10.1 / 9.6; 4 x 4096, 16 / 8 heads, window 128 290 / 283.)
+__device__ __forceinline__ void window_stage(uint32_t tacc, uint32_t sub, int r, int chunk, float mul) {
+    uint32_t v[32];
+    tmem_ld_32x32(tacc, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        uint32_t o[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) o[t] = pack_bf16(__uint_as_float(v[8 * k + 2 * t]) * mul, __uint_as_float(v[8 * k + 2 * t + 1]) * mul);
+        st_shared_v4(sub + r * 128 + (((chunk + k) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
+    }
+}
+// The groups that fill a sub-tile, `threads` of them, wait for each other; one stores it. Rows behind the sequence's end are not written.
+__device__ __forceinline__ void window_store(const CUtensorMap& tm, const uint8_t* sub, int barrier, int threads, bool first, bool ok, int x, int row, int b) {
+    fence_proxy_async_smem();
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
+    if (first && ok) {
+        tma_store_3d(&tm, sub, x, row, b);
+        tma_store_commit();
+        tma_store_wait0();
     }
 }
 
@@ -341,7 +366,7 @@ __device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* tm, uint
 // ---------------------------------------------------------------------------- dK / dV
 // One CTA's work: number `lin` of the (kv tile, batch, head) triples; kWindow: of the parts of AttnWindowParts, those of the window first.
 template <bool kWindow>
-__device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUtensorMap& tm_do, const AttnBwdParams& p, uint8_t* smem, int lin) {
+__device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUtensorMap& tm_do, const CUtensorMap& tm_dqkv, const AttnBwdParams& p, uint8_t* smem, int lin) {
     uint8_t* sK = smem;
     uint8_t* sV = smem + kAttnTileBytes;
     uint8_t* sQ = smem + 2 * kAttnTileBytes;   // 2 stages
@@ -615,61 +640,69 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
         // barriers all the same.
         ok = ok && mbar_wait_warp(final_bar, 0, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN);
         const uint32_t stage = smem_u32(smem);
-        if (ok) {
-            tc_fence_after();
-            const int c0 = (grp & 1) * 2;
-            stage_acc_chunk((grp < 2 ? tdK : tdV) + lane_bits, stage + (grp >> 1) * 65536, r, c0);
-            stage_acc_chunk((grp < 2 ? tdK : tdV) + lane_bits, stage + (grp >> 1) * 65536, r, c0 + 1);
-        }
-        if constexpr (kWindow) fence_proxy_async_smem();
-        bar_sync_compute();
-        if constexpr (kWindow) {
-            // a part leaves its two sums as they are staged; the kernel behind this one adds the parts up
-            if (part.slot >= 0) {
-                if (ok && threadIdx.x == 128) {
-                    char* to = reinterpret_cast<char*>(p.partial) + part.slot * 131072ll;
-                    if (lin < p.cut.near_ctas) {
-                        for (int k = 0; k < 8; ++k) bulk_store(to + k * 16384, smem + k * 16384, 16384);
-                    } else {      // behind the window only the sinks' rows are other than zero
-                        const int bytes = seen_sinks(p.win, j * kAttnTile, kAttnTile) * 512;
-                        bulk_store(to, smem, bytes);
-                        bulk_store(to + 65536, smem + 65536, bytes);
-                    }
-                    tma_store_commit();
-                    tma_store_wait0();
+        if (ok) tc_fence_after();
+        if (kWindow && part.slot < 0) {
+            uint8_t* sub = smem + grp * kAttnSub;      // 64 columns of dK or dV
+            const uint32_t acc = (grp < 2 ? tdK : tdV) + lane_bits + (grp & 1) * 64;
+            if (ok) {
+                window_stage(acc, smem_u32(sub), r, 0, grp < 2 ? p.scale : 1.f);
+                window_stage(acc + 32, smem_u32(sub), r, 4, grp < 2 ? p.scale : 1.f);
+            }
+            window_store(tm_dqkv, sub, 1 + grp, 128, (threadIdx.x & 127) == 0, ok, (grp < 2 ? col_k : col_v) + (grp & 1) * 64, j * kAttnTile, b);
+        } else if constexpr (kWindow) {
+            // A part leaves its sums in fp32, of a sinks' tile behind the window the sinks' rows; the kernel behind this one adds the parts up.
+            // (A whole warp reads tensor memory, whichever of its rows leave.)
+            const int rows = lin < p.cut.near_ctas ? kAttnTile : p.win.sinks - j * kAttnTile;
+            if (ok && (r & ~31) < rows) {
+                float* to = p.partial + part.slot * 32768ll + window_part_at(grp >> 1, r, (grp & 1) * 16);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t v[32];
+                    tmem_ld_32x32((grp < 2 ? tdK : tdV) + lane_bits + (grp & 1) * 64 + c * 32, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (r < rows) *reinterpret_cast<uint4*>(to + (c * 8 + k) * 32) = make_uint4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
                 }
-                ok = false;   // nothing else leaves
             }
-        }
-        const long long ld = kWindow ? p.ldq : static_cast<long long>(p.nh + 2 * p.nkv) * kAttnHD;
-        __nv_bfloat16* row0 = p.dqkv + (static_cast<long long>(row_base) + j * kAttnTile) * ld;
-        __nv_bfloat16* const dst[2] = {row0 + col_k, row0 + col_v};
-        const float mul[2] = {p.scale, 1.f};
-        const int first = threadIdx.x - 128;
-        unsigned int* cnt = !kWindow && p.split_heads ? p.chain + (static_cast<long long>(b) * p.nkv + g) * nq + j : nullptr;
-        if (turn > 0 && ok) {
-            // heads of the group add in turn: wait (bounded) until the heads before me are done
-            ok = false;
-            for (uint32_t spin = 0; spin < kSpinLimit && !ok; ++spin) {
-                unsigned int v;
-                asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(cnt) : "memory");
-                ok = v >= static_cast<unsigned int>(turn);
-                if (!ok && spin > 16) __nanosleep(200);
+        } else {
+            if (ok) {
+                const int c0 = (grp & 1) * 2;
+                stage_acc_chunk((grp < 2 ? tdK : tdV) + lane_bits, stage + (grp >> 1) * 65536, r, c0);
+                stage_acc_chunk((grp < 2 ? tdK : tdV) + lane_bits, stage + (grp >> 1) * 65536, r, c0 + 1);
             }
-            if (!ok) atomicCAS(p.status, 0, CAI_DEV_TIMEOUT_ATTN);
-        }
-        if (ok) {
-            // the last of the heads turns the finished sum
-            const float2* rope = !kWindow && p.rope && (!p.split_heads || turn + 1 == rep) ? p.rope + static_cast<long long>(j) * kAttnTile * 64 : nullptr;
-            if constexpr (kWindow) write_staged<false, 4, true>(stage, dst, mul, ld, first, nullptr, p.S - j * kAttnTile);
-            else if (turn == 0) write_staged<false, 4>(stage, dst, mul, ld, first, rope);
-            else write_staged<true, 4>(stage, dst, mul, ld, first, rope);
-        }
-        if (!kWindow && p.split_heads) {
-            __threadfence();
             bar_sync_compute();
-            if (threadIdx.x == 128) {   // first compute thread: everyone's rows are written and fenced
-                asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(cnt), "r"(static_cast<unsigned int>(turn + 1)) : "memory");
+        }
+        if constexpr (!kWindow) {
+            const long long ld = static_cast<long long>(p.nh + 2 * p.nkv) * kAttnHD;
+            __nv_bfloat16* row0 = p.dqkv + (static_cast<long long>(row_base) + j * kAttnTile) * ld;
+            __nv_bfloat16* const dst[2] = {row0 + col_k, row0 + col_v};
+            const float mul[2] = {p.scale, 1.f};
+            const int first = threadIdx.x - 128;
+            unsigned int* cnt = p.split_heads ? p.chain + (static_cast<long long>(b) * p.nkv + g) * nq + j : nullptr;
+            if (turn > 0 && ok) {
+                // heads of the group add in turn: wait (bounded) until the heads before me are done
+                ok = false;
+                for (uint32_t spin = 0; spin < kSpinLimit && !ok; ++spin) {
+                    unsigned int v;
+                    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(cnt) : "memory");
+                    ok = v >= static_cast<unsigned int>(turn);
+                    if (!ok && spin > 16) __nanosleep(200);
+                }
+                if (!ok) atomicCAS(p.status, 0, CAI_DEV_TIMEOUT_ATTN);
+            }
+            if (ok) {
+                // the last of the heads turns the finished sum
+                const float2* rope = p.rope && (!p.split_heads || turn + 1 == rep) ? p.rope + static_cast<long long>(j) * kAttnTile * 64 : nullptr;
+                if (turn == 0) write_staged<false, 4>(stage, dst, mul, ld, first, rope);
+                else write_staged<true, 4>(stage, dst, mul, ld, first, rope);
+            }
+            if (p.split_heads) {
+                __threadfence();
+                bar_sync_compute();
+                if (threadIdx.x == 128) {   // first compute thread: everyone's rows are written and fenced
+                    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(cnt), "r"(static_cast<unsigned int>(turn + 1)) : "memory");
+                }
             }
         }
     }
@@ -684,7 +717,7 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
 
 // ---------------------------------------------------------------------------- dQ
 template <bool kWindow>
-__device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtensorMap& tm_do, const AttnBwdParams& p, uint8_t* smem, int lin) {
+__device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtensorMap& tm_do, const CUtensorMap& tm_dqkv, const AttnBwdParams& p, uint8_t* smem, int lin) {
     uint8_t* sQ = smem;
     uint8_t* sdO = smem + kAttnTileBytes;
     uint8_t* sK = smem + 2 * kAttnTileBytes;  // 3 stages: S runs a step ahead of the dQ that still needs the tile
@@ -896,18 +929,21 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
         }
         ok = ok && mbar_wait_warp(final_bar, 0, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN);
         const uint32_t stage = smem_u32(smem);
-        if (ok) {
-            tc_fence_after();
-            stage_acc_chunk(tdQ + lane_bits, stage, r, grp);
-        }
-        bar_sync_compute();
-        if (ok) {
-            const long long ld = kWindow ? p.ldq : static_cast<long long>(p.nh + 2 * p.nkv) * kAttnHD;
-            __nv_bfloat16* dst0 = p.dqkv + (static_cast<long long>(row_base) + i * kAttnTile) * ld + col_q;
-            __nv_bfloat16* const dst[2] = {dst0, nullptr};
-            const float mul[2] = {p.scale, 0.f};
-            if constexpr (kWindow) write_staged<false, 2, true>(stage, dst, mul, ld, threadIdx.x - 128, nullptr, p.S - i * kAttnTile);
-            else write_staged<false, 2>(stage, dst, mul, ld, threadIdx.x - 128, p.rope ? p.rope + static_cast<long long>(i) * kAttnTile * 64 : nullptr);
+        if (ok) tc_fence_after();
+        if constexpr (kWindow) {
+            uint8_t* sub = smem + (grp >> 1) * kAttnSub;
+            if (ok) window_stage(tdQ + lane_bits + kb, smem_u32(sub), r, (grp & 1) * 4, p.scale);
+            window_store(tm_dqkv, sub, 1 + (grp >> 1), 256, (threadIdx.x & 255) == 128, ok, col_q + (grp >> 1) * 64, i * kAttnTile, b);
+        } else {
+            if (ok) stage_acc_chunk(tdQ + lane_bits, stage, r, grp);
+            bar_sync_compute();
+            if (ok) {
+                const long long ld = static_cast<long long>(p.nh + 2 * p.nkv) * kAttnHD;
+                __nv_bfloat16* dst0 = p.dqkv + (static_cast<long long>(row_base) + i * kAttnTile) * ld + col_q;
+                __nv_bfloat16* const dst[2] = {dst0, nullptr};
+                const float mul[2] = {p.scale, 0.f};
+                write_staged<false, 2>(stage, dst, mul, ld, threadIdx.x - 128, p.rope ? p.rope + static_cast<long long>(i) * kAttnTile * 64 : nullptr);
+            }
         }
     }
 
@@ -928,8 +964,8 @@ __device__ __forceinline__ void attn_dq(const CUtensorMap& tm_qkv, const CUtenso
 // for nobody: they leave their SMs to whatever part of the chain is not there yet.
 template <bool kWindow>
 __global__ void __launch_bounds__(kAttnBwdThreads, 1)
-attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do, const AttnBwdParams p,
-                const int dkdv_ctas) {
+attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_dqkv,
+                const AttnBwdParams p, const int dkdv_ctas) {
     // no room to round the base up: tiles start on swizzle boundaries only if the shared window does (checked)
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023) {
@@ -938,8 +974,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constan
         return;
     }
     const int cta = static_cast<int>(blockIdx.x);
-    if (cta < dkdv_ctas) attn_dkdv<kWindow>(tm_qkv, tm_do, p, smem, cta);
-    else attn_dq<kWindow>(tm_qkv, tm_do, p, smem, cta - dkdv_ctas);
+    if (cta < dkdv_ctas) attn_dkdv<kWindow>(tm_qkv, tm_do, tm_dqkv, p, smem, cta);
+    else attn_dq<kWindow>(tm_qkv, tm_do, tm_dqkv, p, smem, cta - dkdv_ctas);
 }
 
 constexpr int kAttnBwdSmem = 7 * kAttnTileBytes + 2048 + 256;
@@ -958,38 +994,53 @@ int configure_bwd(int dev) {
 
 // ---------------------------------------------------------------------------- the windowed form's parts
 // A key tile's parts added up, in order, to its bf16 rows of dK (times the scale) and dV: those of the window first, head part by head part, then
-// those of the query tiles behind it. Sixteen CTAs a tile, a thread eight columns of one row of one of the two.
+// those of the query tiles behind it. A thread takes four columns of a row, a warp eight rows of sixteen: a line of 128 bytes for each part of four columns, a sector of
+// 32 for each row it writes. (No shared memory: these CTAs wait beside those of the gradients, which have all of it.)
+constexpr int kJoinCtas = 32;       // of a tile
 __global__ void __launch_bounds__(256)
 attn_window_join_kernel(const AttnBwdParams p) {
     grid_dep_begin();
-    const int lin = blockIdx.x >> 4, item = (blockIdx.x & 15) * 256 + threadIdx.x;
+    const int lin = blockIdx.x / kJoinCtas, item = blockIdx.x % kJoinCtas * 256 + threadIdx.x;
     const int heads_all = p.nkv * p.B, j = lin / heads_all, g = lin % heads_all % p.nkv, b = lin % heads_all / p.nkv;
     const int nq = (p.S + kAttnTile - 1) / kAttnTile, near_last = window_last_query_tile(p.win, j, nq);
     const int far = j < p.cut.sink_tiles ? nq - 1 - near_last : 0;      // query tiles behind the window
     if (p.cut.head_parts * p.cut.near_parts == 1 && far <= 0) return;
-    const int which = item >> 11, r = (item >> 4) & 127, c = (item & 15) * 2;
+    const int which = item >> 12, r = ((item >> 8) & 15) * 8 + ((item >> 2) & 7), c = ((item >> 5) & 7) * 4 + (item & 3);
     if (j * kAttnTile + r >= p.S) return;
-    const uint32_t at0 = which * 65536 + r * 512 + ((c ^ (r & 7)) << 4), at1 = which * 65536 + r * 512 + (((c + 1) ^ (r & 7)) << 4);
-    const char* partial = reinterpret_cast<const char*>(p.partial);
+    const float* at = p.partial + window_part_at(which, r, c);
     const int stride = heads_all * p.cut.head_parts;     // slots of one key tile, of one far part
     const int mine = (b * p.nkv + g) * p.cut.head_parts;
-    float4 s0 = make_float4(0.f, 0.f, 0.f, 0.f), s1 = s0;
-    auto add = [&](long long slot) {
-        const float4 a = *reinterpret_cast<const float4*>(partial + slot * 131072 + at0), d = *reinterpret_cast<const float4*>(partial + slot * 131072 + at1);
-        s0.x += a.x; s0.y += a.y; s0.z += a.z; s0.w += a.w;
-        s1.x += d.x; s1.y += d.y; s1.z += d.z; s1.w += d.w;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    // The head parts of each of `pieces`, from slot `first` on, four loads in flight (more of them, or more code, are slower where the kernel is short).
+    auto add = [&](long long first, int pieces) {
+        const int n = pieces * p.cut.head_parts;
+        const float* piece = at + first * 32768;
+        int k = 0;
+#pragma unroll 1
+        for (int done = 0; done < n; done += 4) {
+            float4 a[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                a[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (done + u < n) a[u] = *reinterpret_cast<const float4*>(piece + k * 32768);
+                if (++k == p.cut.head_parts) {
+                    k = 0;
+                    piece += stride * 32768ll;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                s.x += a[u].x; s.y += a[u].y; s.z += a[u].z; s.w += a[u].w;
+            }
+        }
     };
-    for (int n = 0; n < p.cut.near_parts && j + n * p.cut.near_tiles <= near_last; ++n)
-        for (int k = 0; k < p.cut.head_parts; ++k) add((static_cast<long long>(j) * p.cut.near_parts + n) * stride + mine + k);
-    const int parts = far > 0 && j * kAttnTile + r < p.win.sinks ? (far + p.cut.far_tiles - 1) / p.cut.far_tiles : 0;
-    const long long far0 = p.cut.near_slots + static_cast<long long>(j) * p.cut.far_parts * stride + mine;
-#pragma unroll 4
-    for (int f = 0; f < parts; ++f)
-        for (int k = 0; k < p.cut.head_parts; ++k) add(far0 + static_cast<long long>(f) * stride + k);
+    const int near = (near_last - j) / p.cut.near_tiles + 1;
+    add(static_cast<long long>(j) * p.cut.near_parts * stride + mine, near < p.cut.near_parts ? near : p.cut.near_parts);
+    if (far > 0 && j * kAttnTile + r < p.win.sinks)
+        add(p.cut.near_slots + static_cast<long long>(j) * p.cut.far_parts * stride + mine, (far + p.cut.far_tiles - 1) / p.cut.far_tiles);
     const float mul = which ? 1.f : p.scale;
-    const int col = (which ? p.nh + p.nkv + g : p.nh + g) * kAttnHD + c * 4;
-    *reinterpret_cast<uint4*>(p.dqkv + (static_cast<long long>(b) * p.S + j * kAttnTile + r) * p.ldq + col) =
-        make_uint4(pack_bf16(s0.x * mul, s0.y * mul), pack_bf16(s0.z * mul, s0.w * mul), pack_bf16(s1.x * mul, s1.y * mul), pack_bf16(s1.z * mul, s1.w * mul));
+    *reinterpret_cast<uint2*>(p.dqkv + (static_cast<long long>(b) * p.S + j * kAttnTile + r) * p.ldq + (which ? p.nh + p.nkv + g : p.nh + g) * kAttnHD + c * 4) =
+        make_uint2(pack_bf16(s.x * mul, s.y * mul), pack_bf16(s.z * mul, s.w * mul));
 }
 
 // Whole numbers only, so that host and device agree on every size. Cutting is worth it where one CTA's steps would outlast everybody's share of all steps
@@ -1107,7 +1158,7 @@ CAI_API int cai_flash_attn_bwd_rope(const void* qkv, const void* out, const void
     const long long kv_ctas = (parts & 2) ? static_cast<long long>(nq) * (p.split_heads ? nh : nkv) * B : 0;
     const long long q_ctas = (parts & 4) ? static_cast<long long>(nq) * nh * B : 0;
     if (kv_ctas + q_ctas)
-        launch_early(attn_bwd_kernel<false>, static_cast<unsigned>(kv_ctas + q_ctas), kAttnBwdThreads, kAttnBwdSmem, st, tm_qkv, tm_do, p,
+        launch_early(attn_bwd_kernel<false>, static_cast<unsigned>(kv_ctas + q_ctas), kAttnBwdThreads, kAttnBwdSmem, st, tm_qkv, tm_do, tm_do, p,
                      static_cast<int>(kv_ctas));
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) {
@@ -1157,9 +1208,10 @@ CAI_API int cai_flash_attn_window_bwd(const void* qkv, long long ld, const void*
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const long long ldo = static_cast<long long>(nh) * hd;
-    CUtensorMap tm_qkv, tm_do;
+    CUtensorMap tm_qkv, tm_do, tm_dqkv;
     if (!encode_tmap_3d(&tm_qkv, qkv, static_cast<uint64_t>(nh + 2 * nkv) * hd, S, B, ld, static_cast<uint64_t>(ld) * S, 64, kAttnTile, 2) ||
-        !encode_tmap_3d(&tm_do, dout, ldo, S, B, ldo, static_cast<uint64_t>(ldo) * S, 64, kAttnTile, 2))
+        !encode_tmap_3d(&tm_do, dout, ldo, S, B, ldo, static_cast<uint64_t>(ldo) * S, 64, kAttnTile, 2) ||
+        !encode_tmap_3d(&tm_dqkv, dqkv, static_cast<uint64_t>(nh + 2 * nkv) * hd, S, B, ldq, static_cast<uint64_t>(ldq) * S, 64, kAttnTile, 2))
         return CAI_K_BAD_ARG;
     const int dev = current_device();
     if (configure_bwd<true>(dev)) return CAI_K_CUDA;
@@ -1187,10 +1239,10 @@ CAI_API int cai_flash_attn_window_bwd(const void* qkv, long long ld, const void*
     const int kv_ctas = p.cut.near_ctas + p.cut.far_ctas;
     const long long q_ctas = static_cast<long long>((S + kAttnTile - 1) / kAttnTile) * nh * B;
     if (e == cudaSuccess)
-        e = launch_early(attn_bwd_kernel<true>, static_cast<unsigned>(kv_ctas + q_ctas), kAttnBwdThreads, kAttnBwdSmem, st, tm_qkv, tm_do, p, kv_ctas);
+        e = launch_early(attn_bwd_kernel<true>, static_cast<unsigned>(kv_ctas + q_ctas), kAttnBwdThreads, kAttnBwdSmem, st, tm_qkv, tm_do, tm_dqkv, p, kv_ctas);
     if (e == cudaSuccess && p.cut.near_slots + p.cut.far_ctas > 0) {
         const long long tiles = p.cut.head_parts * p.cut.near_parts > 1 ? (S + kAttnTile - 1) / kAttnTile : p.cut.sink_tiles;
-        e = launch_early(attn_window_join_kernel, static_cast<unsigned>(tiles * nkv * B * 16), 256, 0, st, p);
+        e = launch_early(attn_window_join_kernel, static_cast<unsigned>(tiles * nkv * B * kJoinCtas), 256, 0, st, p);
     }
     if (e != cudaSuccess) {
         set_last_error("flash_attn_window_bwd launch failed: %s", cudaGetErrorString(e));
