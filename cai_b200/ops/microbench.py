@@ -7,6 +7,9 @@ iterations). Also the small fixed-size workloads that profiler captures are take
     python -m cai_b200.ops.microbench rmsnorm_bwd --rows 4096 --hidden 2048
     python -m cai_b200.ops.microbench swiglu --rows 4096 --ffn 8192
     python -m cai_b200.ops.microbench gemm_fp8 --m 8192 --n 8192 --k 8192
+    python -m cai_b200.ops.microbench window_fwd --batch 4 --seq 4096 --heads 16 --kv-heads 8 --window 1024 --sinks 4     (window_bwd likewise)
+    python -m cai_b200.ops.microbench norm_quant --rows 16384 --hidden 4096       (with residual and y)
+    python -m cai_b200.ops.microbench rope_axes --rows 32768 --heads 32 --kv-heads 8
     python -m cai_b200.ops.microbench gemm_swiglu --m 8192 --n 16384 --k 2048     (n = 2 x ffn: gate and up)
 
 Prints one JSON line per run: milliseconds (median of ``--iters`` after ``--warmup``), achieved
@@ -21,7 +24,8 @@ from pathlib import Path
 
 import torch
 
-from . import (flash_attn_bwd, flash_attn_fwd, gemm, rmsnorm_bwd, rmsnorm_fwd, swiglu_bwd, swiglu_fwd)
+from . import (add_rmsnorm_quant, flash_attn_bwd, flash_attn_fwd, flash_attn_window_bwd, flash_attn_window_fwd, gemm, rmsnorm_bwd, rmsnorm_fwd, rope_apply_axes_,
+               rope_freqs, swiglu_bwd, swiglu_fwd)
 
 ROOT = Path(__file__).resolve().parent.parent.parent
 
@@ -53,7 +57,8 @@ def timeit(fn, iters, warmup, flush):
 
 def main(argv=None):
     ap = argparse.ArgumentParser()
-    ap.add_argument("kernel", choices=["gemm", "gemm_fp8", "gemm_swiglu", "attn_fwd", "attn_bwd", "rmsnorm_bwd", "swiglu"])
+    ap.add_argument("kernel", choices=["gemm", "gemm_fp8", "gemm_swiglu", "attn_fwd", "attn_bwd", "window_fwd", "window_bwd", "norm_quant", "rope_axes",
+                                       "rmsnorm_bwd", "swiglu"])
     ap.add_argument("--m", type=int, default=8192)
     ap.add_argument("--n", type=int, default=8192)
     ap.add_argument("--k", type=int, default=8192)
@@ -64,6 +69,8 @@ def main(argv=None):
     ap.add_argument("--seq", type=int, default=4096)
     ap.add_argument("--heads", type=int, default=16)
     ap.add_argument("--kv-heads", type=int, default=8)
+    ap.add_argument("--window", type=int, default=1024)
+    ap.add_argument("--sinks", type=int, default=4)
     ap.add_argument("--rows", type=int, default=4096)
     ap.add_argument("--hidden", type=int, default=2048)
     ap.add_argument("--ffn", type=int, default=8192)
@@ -123,6 +130,36 @@ def main(argv=None):
         tf = flops / ms / 1e9
         out.update(batch=a.batch, seq=a.seq, heads=a.heads, kv_heads=a.kv_heads, ms=ms, tflops_useful=tf,
                    frac_of_peak=tf / tf_peak, peak_source=src)
+    elif a.kernel in ("window_fwd", "window_bwd"):
+        hd = 128
+        shape = (a.batch, a.seq, a.heads, a.kv_heads, hd, a.window, a.sinks)
+        qkv = torch.randn(a.batch * a.seq, (a.heads + 2 * a.kv_heads) * hd, device=dev).to(bf)
+        o, lse = flash_attn_window_fwd(qkv, *shape)
+        i = torch.arange(a.seq)
+        lo = (i - a.window + 1).clamp_min(0)      # of the window's first key
+        pairs = a.batch * a.heads * int((i + 1 - lo + lo.clamp_max(a.sinks)).sum())
+        if a.kernel == "window_fwd":
+            ms = timeit(lambda: flash_attn_window_fwd(qkv, *shape), a.iters, a.warmup, flush)
+        else:
+            do, dqkv = torch.randn_like(o), torch.empty_like(qkv)
+            ms = timeit(lambda: flash_attn_window_bwd(qkv, o, do, lse, *shape, dqkv=dqkv), a.iters, a.warmup, flush)
+        tf = (4.0 if a.kernel == "window_fwd" else 10.0) * hd * pairs / ms / 1e9
+        out.update(batch=a.batch, seq=a.seq, heads=a.heads, kv_heads=a.kv_heads, window=a.window, sinks=a.sinks, ms=ms, tflops_useful=tf,
+                   frac_of_peak=tf / tf_peak, peak_source=src)
+    elif a.kernel == "norm_quant":
+        x, r = torch.randn(a.rows, a.hidden, device=dev).to(bf), torch.randn(a.rows, a.hidden, device=dev).to(bf)
+        g = torch.ones(a.hidden, device=dev, dtype=bf)
+        ms = timeit(lambda: add_rmsnorm_quant(x, r, g, keep_y=True), a.iters, a.warmup, flush)
+        gb = 9.0 * a.rows * a.hidden / 1e9       # x, residual in; h, y, q out
+        out.update(rows=a.rows, hidden=a.hidden, ms=ms, gbs=gb / (ms * 1e-3), frac_of_peak=gb / (ms * 1e-3) / bw_peak, peak_source=src)
+    elif a.kernel == "rope_axes":
+        hd = 128
+        qkv = torch.randn(a.rows, (a.heads + 2 * a.kv_heads) * hd, device=dev).to(bf)
+        pos = torch.randint(0, 4096, (3, a.rows), device=dev, dtype=torch.int32)
+        freqs = rope_freqs(hd, device=dev)
+        ms = timeit(lambda: rope_apply_axes_(qkv, freqs, pos, a.heads, a.kv_heads, hd, (24, 20, 20)), a.iters, a.warmup, flush)
+        gb = 4.0 * a.rows * (a.heads + a.kv_heads) * hd / 1e9
+        out.update(rows=a.rows, heads=a.heads, kv_heads=a.kv_heads, ms=ms, gbs=gb / (ms * 1e-3), frac_of_peak=gb / (ms * 1e-3) / bw_peak, peak_source=src)
     elif a.kernel == "rmsnorm_bwd":
         x = torch.randn(a.rows, a.hidden, device=dev).to(bf)
         g = torch.ones(a.hidden, device=dev, dtype=bf)
