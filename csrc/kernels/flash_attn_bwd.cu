@@ -36,6 +36,13 @@
 // P^T over S^T in TMEM, with S^T(i+1) behind dV(i): 8 % slower. Asking the barriers early without blocking, and fetching
 // the next scores before dS^T is handed over: 2-10 % slower.
 //
+// The windowed form (kWindow; a window and sinks, sequences of any length) is the same two parts over lists of tiles: of dK / dV the query tiles that see a key tile, of dQ the key
+// tiles that a query tile sees. It cuts dK / dV's sums into parts that a third kernel adds up in a fixed order (AttnWindowParts): over heads and query tiles in small
+// grids, and the sinks' sums, which run over all later queries. Tensor maps with the sequences apart bring rows past a sequence's end as zeros and leave them out of the
+// result. Warps that see nothing of a tile skip its exponentials. us: 4 x 4096 tokens, 16 / 8 heads, 4 sinks, window 1024 540 in a burst, 590 back to back at the power
+// limit (985 W, 1657-1725 MHz; 560 TFLOP/s of the five products of what is seen; seven are computed), window 128 280; 16384 tokens, window 4096 1680; 333 tokens, 8 / 1 heads 14.4, 2 x 128,
+// 2 / 1 heads 9.7. dQ from the same scores as dK / dV, added to in L2 in a fixed order, took 725 against 600: the additions go at some 30 bytes a cycle and SM.
+//
 // Replaces the reference's one-thread-per-query backward, which recomputes dp twice, scatters
 // dK/dV with atomicAdd and never zeroes dq/dk/dv (src/cuda/cai_kernels.cu:110-143).
 #include <math.h>

@@ -5,6 +5,8 @@
 //
 // The norm is that of the rounded h, which is what the backward pass reads; q is rounded once, from y in fp32 (through a bf16 y, as the two kernels of
 // their own do it, values next to a border of e4m3 are rounded twice).
+// Measured on a B200: 16384 x 4096 with residual and y 89 us (9 bytes an element, 6.8 TB/s: the rate of a copy), without either 48 (3 bytes, 4.2 TB/s, bound by
+// instructions), 8192 x 2048 24.7, 1777 x 1408 without either 3.8, 256 x 256 1.8, where a launch's own latencies are all there is.
 #include <cuda_fp8.h>
 
 #include "cai_kernels.h"

@@ -2,7 +2,8 @@
 //
 // Pair i of a head, its elements i and i + half, is turned by pos[axis(i)][token] * freqs[i]. The product is taken in 64 bits and brought to a part of
 // one turn there: in 32 bits an angle of 10^5 radians is off by 0.004, as much as the result's rounding. A pair's angle is computed once per token, not
-// once per head.
+// once per head. Bound by memory, four bytes an element of q and k. Measured on a B200: 32768 tokens of 32 / 8 heads 101 us (6.7 TB/s: the rate of a copy), 5003 of
+// 9 / 3 heads 4.9, 256 of 2 / 1 1.9.
 #include "cai_kernels.h"
 #include "host_common.h"
 #include "norm_kernels.cuh"
