@@ -1051,7 +1051,7 @@ attn_window_join_kernel(const AttnBwdParams p) {
 }
 
 // Whole numbers only, so that host and device agree on every size. Cutting is worth it where one CTA's steps would outlast everybody's share of all steps
-// by more than the second kernel costs, which is that of three steps and a little for each part it reads: dK / dV of a step cost about 5 / 4 of dQ's. us of a
+// by more than the second kernel costs, which is that of two steps and a little for each part it reads: dK / dV of a step cost about 5 / 4 of dQ's. us of a
 // backward, whole tiles or cut by heads / by heads and query tiles: 4000 tokens, 1 head 63 / 51, 2 x 1500, 8 / 1 heads, window 100 38 / 35, 2000, 4 / 4 36 /
 // 33, 5 x 60, 24 / 3 22 / 18.
 AttnWindowParts window_parts(const AttnWindow& w, int B, int S, int nh, int nkv, int sms) {
@@ -1069,7 +1069,7 @@ AttnWindowParts window_parts(const AttnWindow& w, int B, int S, int nh, int nkv,
         for (int near = 1; rep % heads == 0 && near <= near_most; near *= 2) {
             const int tiles = (near_most + near - 1) / near;
             const long long longest = 5ll * tiles * (rep / heads), slots = groups * nq * heads * near;
-            const long long cost = (longest > share ? longest : share) + (heads * near > 1 ? (c.sink_tiles ? 0 : 12) + slots / 8 : 0);
+            const long long cost = (longest > share ? longest : share) + (heads * near > 1 ? (c.sink_tiles ? 0 : 8) + slots / 8 : 0);
             if (best >= 0 && cost >= best) continue;
             best = cost;
             c.head_parts = heads;

@@ -250,6 +250,20 @@ def test_workspaces_given_and_streams_side_by_side():
         ops.flash_attn_window_bwd(a[0][0], *fwd[0][:1], a[0][1], fwd[0][1], B, S, nh, nkv, HD, window, sinks, scratch=work[0][1][1:])
 
 
+@pytest.mark.parametrize("B,S,nh,nkv,window,sinks", [(1, 900, 2, 1, 900, 0), (1, 4000, 1, 1, 4000, 0), (2, 1500, 8, 1, 100, 100), (1, 333, 8, 1, 512, 1), (1, 6000, 2, 2, 1000, 17),
+                                                     (1, 129, 32, 8, 129, 1), (1, 5000, 4, 2, 300, 257)])
+def test_what_the_scratch_held_does_not_matter(B, S, nh, nkv, window, sinks):
+    """Sums cut over heads, over query tiles, over both, and the sinks' rows alone: what is joined is what the parts wrote."""
+    from cai_b200 import ops
+    qkv, dout = _inputs(B, S, nh, nkv, 5)
+    out, lse = ops.flash_attn_window_fwd(qkv, B, S, nh, nkv, HD, window, sinks)
+    need = ops.flash_attn_window_bwd_scratch(B, S, nh, nkv, window, sinks)
+    assert need > 0
+    got = [ops.flash_attn_window_bwd(qkv, out, dout, lse, B, S, nh, nkv, HD, window, sinks, scratch=torch.full((need // 4,), v, device="cuda"),
+                                     dqkv=torch.full_like(qkv, v)) for v in (float("nan"), 0.0)]
+    assert got[0].isfinite().all() and torch.equal(*got)
+
+
 def test_captured_and_replayed():
     from cai_b200 import ops
     B, S, nh, nkv, window, sinks = 2, 700, 4, 1, 130, 3
