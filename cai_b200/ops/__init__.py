@@ -174,7 +174,8 @@ def add_rmsnorm_quant(x, residual, g, eps=1e-6, *, keep_y=False):
 
     ``x`` and ``residual`` are bf16 ``[rows, H]`` of any row pitch that is a multiple of 8, ``H`` a multiple of 128 up to 16384; ``g`` bf16 ``[H]``. Returns
     ``(h, q, s, rstd, y)``: ``h`` bf16 (``x`` itself where ``residual`` is None), ``q`` e4m3 ``[rows, H]``, ``s`` f32 ``[rows, H / 128]``, ``rstd`` f32
-    ``[rows]``, ``y`` bf16, or None without ``keep_y`` (a weight gradient reads it). ``q`` is rounded once, from y in fp32. The gradients are
+    ``[rows]``, ``y`` bf16, or None without ``keep_y`` (a weight gradient reads it); h, y and rstd share an allocation, q and s another. ``q`` is rounded once,
+    from y in fp32. The gradients are
     ``rmsnorm_bwd(h, g, rstd, dy, dx=dh, dx_accumulate=True)``: ``dh``, the gradient of ``h`` that comes past the norm, becomes that of x and of residual."""
     return native().add_rmsnorm_quant(x, residual, g, eps, keep_y)
 
@@ -282,7 +283,8 @@ def flash_attn_bwd(qkv, out, dout, lse, B, S, nh, nkv, hd, scale=None, dqkv=None
 def flash_attn_window_fwd(qkv, B, S, nh, nkv, hd, window, sinks=0, scale=None):
     """Causal GQA flash attention with a window and sinks over packed ``qkv`` ``[B*S, (nh + 2 nkv) * hd]`` (bf16, any row pitch that is a multiple of 8): query i
     sees key j if ``j <= i`` and (``j > i - window`` or ``j < sinks``). Any ``S``; ``window >= 1``, ``sinks >= 0``, head_dim 128. Returns ``out`` bf16
-    ``[B*S, nh * hd]`` and ``lse`` f32 ``[B, nh, S]``."""
+    ``[B*S, nh * hd]`` and ``lse`` f32 ``[B, nh, S]``, which share an allocation. All of ``qkv`` has to be
+    finite: a value that is not reaches queries of its tile that do not see it, though not another sequence."""
     return native().flash_attn_window_fwd(qkv, B, S, nh, nkv, hd, window, sinks, scale)
 
 

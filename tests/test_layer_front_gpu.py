@@ -79,6 +79,37 @@ def test_norm_results_are_apart(rows, H):
     assert torch.equal(s, want[2]) and torch.equal(rstd, want[3]) and len(other) == 8
 
 
+def test_norm_of_no_rows():
+    from cai_b200 import ops
+    x, g = torch.zeros(0, 256, device="cuda", dtype=torch.bfloat16), torch.ones(256, device="cuda", dtype=torch.bfloat16)
+    for r, keep in ((x, True), (None, False)):
+        h, q, s, rstd, y = ops.add_rmsnorm_quant(x, r, g, keep_y=keep)
+        assert h.shape == (0, 256) and q.shape == (0, 256) and s.shape == (0, 2) and rstd.shape == (0,) and (y is None or y.shape == (0, 256))
+
+
+def test_results_are_freed_and_handed_to_streams():
+    """What a call returns is freed when the last of what shares its memory goes, and may be recorded on another stream."""
+    from cai_b200 import ops
+    x, r, g = _norm_inputs(4096, 1024, 2)
+    ops.add_rmsnorm_quant(x, r, g, keep_y=True)
+    torch.cuda.synchronize()
+    before, side = torch.cuda.memory_allocated(), torch.cuda.Stream()
+    got = ops.add_rmsnorm_quant(x, r, g, keep_y=True)
+    want = got[2].clone()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kept = got[2].clone()
+    got[2].record_stream(side)
+    assert torch.cuda.memory_allocated() > before
+    del got
+    torch.cuda.synchronize()
+    assert torch.equal(kept, want)
+    del kept, want
+    torch.cuda.synchronize()
+    torch.zeros(1, device="cuda")          # the allocator looks at what has been recorded
+    assert torch.cuda.memory_allocated() <= before
+
+
 def test_norm_of_views():
     """Rows with pitches of their own, a residual that is one row for all, rows that start in the middle of a buffer of NaN."""
     from cai_b200 import ops
