@@ -110,6 +110,26 @@ def test_results_are_freed_and_handed_to_streams():
     assert torch.cuda.memory_allocated() <= before
 
 
+def test_offsets_beyond_32_bits():
+    from cai_b200 import ops
+    rows, H = 300 * 1024, 8192
+    assert rows * H > 1 << 31
+    x, r, g = _norm_inputs(1024, H, 12)
+    X, R = x.repeat(300, 1), r.repeat(300, 1)
+    want, got = ops.add_rmsnorm_quant(x, r, g, keep_y=True), ops.add_rmsnorm_quant(X, R, g, keep_y=True)
+    for a, b in zip(want, got):
+        assert torch.equal(a.view(torch.uint8), b[-1024:].view(torch.uint8)) and torch.equal(a.view(torch.uint8), b[150 * 1024:151 * 1024].view(torch.uint8))
+    del X, R, got, want
+    T, nh, nkv = 384 * 1024, 40, 4
+    qkv = torch.randn(4096, 48 * 128, device="cuda").to(torch.bfloat16)
+    pos, freqs = torch.randint(0, 5000, (2, 4096), device="cuda", dtype=torch.int32), ops.rope_freqs(128)
+    big = qkv.repeat(T // 4096, 1)
+    assert big.numel() > 1 << 31
+    ops.rope_apply_axes_(big, freqs, pos.repeat(1, T // 4096), nh, nkv, 128, (32, 32))
+    ops.rope_apply_axes_(qkv, freqs, pos, nh, nkv, 128, (32, 32))
+    assert torch.equal(big[-4096:], qkv)
+
+
 def test_norm_of_views():
     """Rows with pitches of their own, a residual that is one row for all, rows that start in the middle of a buffer of NaN."""
     from cai_b200 import ops

@@ -69,7 +69,8 @@ def _inputs(B, S, nh, nkv, seed=0, size=1.0):
 
 SHAPES = [(1, 1, 1, 1, 1, 0), (3, 1, 4, 2, 5, 3), (2, 5, 2, 1, 2, 1), (1, 127, 3, 1, 128, 0), (2, 128, 2, 2, 1, 0), (1, 129, 4, 1, 64, 4), (2, 200, 8, 1, 37, 130),
           (1, 300, 2, 1, 300, 300), (1, 513, 6, 2, 128, 1), (2, 640, 4, 4, 129, 127), (1, 1000, 9, 3, 200, 0), (1, 1300, 4, 1, 16, 129), (1, 1111, 16, 2, 4096, 5),
-          (5, 256, 3, 3, 255, 256), (30, 384, 3, 1, 100, 2), (1, 2049, 4, 2, 640, 64), (1, 3000, 2, 1, 50, 1)]
+          (5, 256, 3, 3, 255, 256), (30, 384, 3, 1, 100, 2), (1, 2049, 4, 2, 640, 64), (1, 3000, 2, 1, 50, 1), (65535, 2, 2, 1, 2, 1), (1, 150, 128, 1, 40, 2),
+          (1, 128, 32, 8, 128, 1), (1, 333, 8, 1, 512, 1)]
 
 
 @pytest.mark.parametrize("B,S,nh,nkv,window,sinks", SHAPES)
@@ -262,6 +263,27 @@ def test_what_the_scratch_held_does_not_matter(B, S, nh, nkv, window, sinks):
     got = [ops.flash_attn_window_bwd(qkv, out, dout, lse, B, S, nh, nkv, HD, window, sinks, scratch=torch.full((need // 4,), v, device="cuda"),
                                      dqkv=torch.full_like(qkv, v)) for v in (float("nan"), 0.0)]
     assert got[0].isfinite().all() and torch.equal(*got)
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 elements in one sequence: its end gives what the end alone gives, bit for bit (the cut lies at a tile's beginning)."""
+    from cai_b200 import ops
+    S, nh, nkv, window, tail = 384 * 1024, 32, 8, 200, 2048
+    cols = (nh + 2 * nkv) * HD
+    assert S * cols > 1 << 31
+    g = torch.Generator(device="cuda").manual_seed(3)
+    piece = torch.randn(4096, cols, device="cuda", generator=g).to(torch.bfloat16)
+    qkv = piece.repeat(S // 4096, 1)
+    dout = torch.randn(4096, nh * HD, device="cuda", generator=g).to(torch.bfloat16).repeat(S // 4096, 1)
+    out, lse = ops.flash_attn_window_fwd(qkv, 1, S, nh, nkv, HD, window)
+    q, d = qkv[S - tail:].contiguous(), dout[S - tail:].contiguous()
+    o, l = ops.flash_attn_window_fwd(q, 1, tail, nh, nkv, HD, window)
+    assert torch.equal(out[S - tail + window:], o[window:]) and torch.equal(lse[..., S - tail + window:], l[..., window:])
+    dqkv = ops.flash_attn_window_bwd(qkv, out, dout, lse, 1, S, nh, nkv, HD, window)
+    dq = ops.flash_attn_window_bwd(q, o, d, l, 1, tail, nh, nkv, HD, window)
+    # (sums may be cut otherwise in the short call: their order is that of fp32 additions, their result is rounded once)
+    a, b = dqkv[S - tail + window:].float(), dq[window:].float()
+    assert ((a - b).abs() <= 2 * HALF * b.abs() + SLACK * b.abs().amax()).all()
 
 
 def test_captured_and_replayed():
