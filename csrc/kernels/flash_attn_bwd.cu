@@ -999,6 +999,99 @@ int configure_bwd(int dev) {
     return CAI_K_OK;
 }
 
+// ---------------------------------------------------------------------------- the windowed form's row sums
+// sum_d dO O has the rounding of O in it, and dS = P (dP - delta) is a difference: where a query sees few keys, what O was rounded by counts for more than what dS is (of two
+// keys dq and dk were off by 2.5 roundings, of sixteen by 1.55, of a hundred by 1.48, 1.41 being P's or dS's and the result's own). So there delta is sum_j P dP,
+// which it stands for, in fp32: a warp takes sixteen queries of a head and eight keys at a time, with the warp's own matrix instruction (a tile of 128 x 128 would be
+// seen to an eighth and less). The order of the head's dimension inside a product is free: a lane takes eight of them in a row, of queries and of keys.
+// kFewKeys: seen by a query at most; kFewRows: of a sequence, whose early queries see few whatever the window is. In small grids the four warps of a CTA share the keys of one
+// piece (`ways`): the time is one warp's chain of loads and exponentials. us of a backward, so / from O: 4 x 4096 tokens, 16 / 8 heads, window 8 239 / 216, 3 x 1000, 9 / 3 heads,
+// window 20 33.4 / 30.4 (four ways 37.8), 96 tokens, 8 / 2 heads 12.1 / 10.4 (one way 16.0).
+constexpr int kFewKeys = 24, kFewRows = 96;
+__device__ __forceinline__ void mma_16x8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__global__ void __launch_bounds__(128, 4)
+attn_window_row_sums_kernel(const __nv_bfloat16* __restrict__ qkv, long long ld, const __nv_bfloat16* __restrict__ dout, const float* __restrict__ lse,
+                            float* __restrict__ delta, int B, int S, int nh, int nkv, float scale_log2, AttnWindow win, int ways) {
+    __shared__ float sums[4][16];
+    grid_dep_begin();
+    // heads fastest: those of a kv head read the same keys
+    const int pieces = (S + 15) / 16, lane = threadIdx.x & 31, row = lane >> 2, part = lane & 3;
+    const int warp = threadIdx.x >> 5, mine = ways == 4 ? warp : 0;
+    const long long item = ways == 4 ? blockIdx.x : static_cast<long long>(blockIdx.x) * 4 + warp;
+    if (item >= static_cast<long long>(pieces) * nh * B) return;
+    const int h = static_cast<int>(item % nh), q0 = static_cast<int>(item / nh % pieces) * 16, b = static_cast<int>(item / nh / pieces), g = h / (nh / nkv);
+    const long long first = static_cast<long long>(b) * S;
+    uint4 q[2][4], d[2][4];
+    float neg_lse2[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int at = q0 + row + u * 8;
+        const bool there = at < S;
+        neg_lse2[u] = there ? lse[(static_cast<long long>(b) * nh + h) * S + at] * -1.4426950408889634f : -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            q[u][c] = d[u][c] = make_uint4(0, 0, 0, 0);
+            if (there) {
+                q[u][c] = *reinterpret_cast<const uint4*>(qkv + (first + at) * ld + h * kAttnHD + c * 32 + part * 8);
+                d[u][c] = *reinterpret_cast<const uint4*>(dout + ((first + at) * nh + h) * kAttnHD + c * 32 + part * 8);
+            }
+        }
+    }
+    auto keys = [&](int k0) {
+        const int at = k0 + row;
+        float s[4] = {}, dp[4] = {};
+        const __nv_bfloat16* k = qkv + (first + at) * ld + (nh + g) * kAttnHD + part * 8;
+        const __nv_bfloat16* v = k + nkv * kAttnHD;
+        uint4 kk[4], vv[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            kk[c] = vv[c] = make_uint4(0, 0, 0, 0);
+            if (at < S) {
+                kk[c] = *reinterpret_cast<const uint4*>(k + c * 32);
+                vv[c] = *reinterpret_cast<const uint4*>(v + c * 32);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            mma_16x8(s, q[0][c].x, q[1][c].x, q[0][c].y, q[1][c].y, kk[c].x, kk[c].y);
+            mma_16x8(s, q[0][c].z, q[1][c].z, q[0][c].w, q[1][c].w, kk[c].z, kk[c].w);
+            mma_16x8(dp, d[0][c].x, d[1][c].x, d[0][c].y, d[1][c].y, vv[c].x, vv[c].y);
+            mma_16x8(dp, d[0][c].z, d[1][c].z, d[0][c].w, d[1][c].w, vv[c].z, vv[c].w);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = q0 + row + (e >> 1) * 8, j = k0 + part * 2 + (e & 1);
+            if (j <= i && (j > i - win.window || j < win.sinks)) sum[e >> 1] += fast_exp2(s[e] * scale_log2 + neg_lse2[e >> 1]) * dp[e];
+        }
+    };
+    const int reach = q0 - win.window + 1, near = (reach > 0 ? reach : 0) & ~7, last = q0 + 15 < S - 1 ? q0 + 15 : S - 1;
+    const int sinks = win.sinks < near ? win.sinks : near;
+    for (int k0 = mine * 8; k0 < sinks; k0 += ways * 8) keys(k0);
+    for (int k0 = near + mine * 8; k0 <= last; k0 += ways * 8) keys(k0);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 1);
+        sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 2);
+    }
+    float* out = delta + (static_cast<long long>(b) * nh + h) * S + q0;
+    if (ways == 4) {
+        if (part == 0) {
+            sums[warp][row] = sum[0];
+            sums[warp][row + 8] = sum[1];
+        }
+        __syncthreads();
+        if (threadIdx.x < 16 && q0 + threadIdx.x < S)
+            out[threadIdx.x] = sums[0][threadIdx.x] + sums[1][threadIdx.x] + sums[2][threadIdx.x] + sums[3][threadIdx.x];
+    } else if (part == 0) {
+        if (q0 + row < S) out[row] = sum[0];
+        if (q0 + row + 8 < S) out[row + 8] = sum[1];
+    }
+}
+
 // ---------------------------------------------------------------------------- the windowed form's parts
 // A key tile's parts added up, in order, to its bf16 rows of dK (times the scale) and dV: those of the window first, head part by head part, then
 // those of the query tiles behind it. A thread takes four columns of a row, a warp eight rows of sixteen: a line of 128 bytes for each part of four columns, a sector of
@@ -1239,10 +1332,18 @@ CAI_API int cai_flash_attn_window_bwd(const void* qkv, long long ld, const void*
         return CAI_K_BAD_ARG;
     }
     const long long rows = static_cast<long long>(B) * S * nh;
-    constexpr unsigned per_cta = 16u * kDeltaUnroll;
-    cudaError_t e = launch_early(attn_delta_kernel, static_cast<unsigned>((rows + per_cta - 1) / per_cta), 256, 0, st,
-                                 static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(dout), delta, static_cast<unsigned>(rows),
-                                 static_cast<unsigned>(S), static_cast<unsigned>(nh), true, static_cast<unsigned int*>(nullptr), 0u);
+    cudaError_t e;
+    if (S <= kFewRows || static_cast<long long>(p.win.window) + p.win.sinks <= kFewKeys) {
+        const long long pieces = static_cast<long long>((S + 15) / 16) * nh * B;
+        const int ways = pieces < 4 * sm_count(dev) ? 4 : 1;
+        e = launch_early(attn_window_row_sums_kernel, static_cast<unsigned>((pieces * ways + 3) / 4), 128, 0, st, static_cast<const __nv_bfloat16*>(qkv), ld,
+                         static_cast<const __nv_bfloat16*>(dout), lse, delta, B, S, nh, nkv, p.scale_log2, p.win, ways);
+    } else {
+        constexpr unsigned per_cta = 16u * kDeltaUnroll;
+        e = launch_early(attn_delta_kernel, static_cast<unsigned>((rows + per_cta - 1) / per_cta), 256, 0, st,
+                         static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(dout), delta, static_cast<unsigned>(rows),
+                         static_cast<unsigned>(S), static_cast<unsigned>(nh), true, static_cast<unsigned int*>(nullptr), 0u);
+    }
     const int kv_ctas = p.cut.near_ctas + p.cut.far_ctas;
     const long long q_ctas = static_cast<long long>((S + kAttnTile - 1) / kAttnTile) * nh * B;
     if (e == cudaSuccess)
