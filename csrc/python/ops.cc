@@ -37,13 +37,17 @@ void need(bool ok, const char* op, const char* what) {
 void launched(int rc, const char* op) {
     if (__builtin_expect(rc != 0, 0)) throw Refused(std::string(op) + " failed (rc=" + std::to_string(rc) + "): " + cai_last_error());
 }
-// A launch waits when the stream's queue is full: others may run meanwhile.
+// A launch waits when the stream's queue is full: others may run meanwhile. What is thrown meanwhile finds the thread's state restored; tensors are asked for their
+// addresses before, since that is what throws (under torch.vmap they have none).
+struct WithoutGil {
+    PyThreadState* const state = PyEval_SaveThread();
+    WithoutGil() = default;
+    WithoutGil(const WithoutGil&) = delete;
+    ~WithoutGil() { PyEval_RestoreThread(state); }
+};
 template <typename F> int without_gil(F&& f) {
-    int rc;
-    Py_BEGIN_ALLOW_THREADS
-    rc = f();
-    Py_END_ALLOW_THREADS
-    return rc;
+    const WithoutGil released;
+    return f();
 }
 
 // ---------------------------------------------------------------- arguments
@@ -156,9 +160,12 @@ PyObject* add_rmsnorm_quant(PyObject* const* a) {
     Piece kept(rows * H * 2 * ((residual != nullptr) + keep_y) + rows * 4), read(rows * H + rows * (H / 128) * 4);
     const at::Tensor h = residual ? kept.make(at::kBFloat16, {rows, H}) : at::Tensor(), y = keep_y ? kept.make(at::kBFloat16, {rows, H}) : at::Tensor();
     const at::Tensor rstd = kept.make(at::kFloat, {rows}), q = read.make(at::kFloat8_e4m3fn, {rows, H}), s = read.make(at::kFloat, {rows, H / 128});
+    const int64_t ldx = rows > 1 ? x.stride(0) : 0, ldr = residual && rows > 1 ? residual->stride(0) : 0;
+    const void *xp = p(x), *rp = residual ? p(*residual) : nullptr, *gp = p(g);
+    void *hp = p(h), *yp = p(y), *qp = p(q);
+    float *sp = p<float>(s), *rstdp = p<float>(rstd);
     launched(without_gil([&] {
-        return cai_add_rmsnorm_quant(p(x), rows > 1 ? x.stride(0) : 0, residual ? p(*residual) : nullptr, residual && rows > 1 ? residual->stride(0) : 0, p(g), p(h),
-                                     p(y), p(q), p<float>(s), p<float>(rstd), static_cast<int>(rows), static_cast<int>(H), eps, at.stream);
+        return cai_add_rmsnorm_quant(xp, ldx, rp, ldr, gp, hp, yp, qp, sp, rstdp, static_cast<int>(rows), static_cast<int>(H), eps, at.stream);
     }), op);
     THPObjectPtr out(PyTuple_New(5));
     if (!out) throw Raised();
@@ -190,9 +197,13 @@ PyObject* rope_apply_axes(PyObject* const* a) {
     need(pos.scalar_type() == at::kInt && shaped(pos, axes, T) && (T < 2 || pos.stride(1) == 1), op, "pos is int32 [axes, T], an axis' positions contiguous");
     need(freqs.scalar_type() == at::kDouble && freqs.dim() == 1 && freqs.size(0) == hd / 2 && freqs.is_contiguous(), op, "freqs is f64 [hd / 2]");
     const Place at = place(op, {&qkv, &freqs, &pos});
+    const int64_t ldp = axes > 1 ? pos.stride(0) : 0, ld = T > 1 ? qkv.stride(0) : (cols + 7) / 8 * 8;
+    void* qkvp = p(qkv);
+    const double* freqsp = p<double>(freqs);
+    const int* posp = p<int>(pos);
     launched(without_gil([&] {
-        return cai_rope_apply_axes(p(qkv), p<double>(freqs), p<int>(pos), axes > 1 ? pos.stride(0) : 0, static_cast<int>(T), nh, nkv, hd,
-                                   T > 1 ? qkv.stride(0) : (cols + 7) / 8 * 8, static_cast<int>(axes), n[0], n[1], n[2], n[3], interleaved, inverse, at.stream);
+        return cai_rope_apply_axes(qkvp, freqsp, posp, ldp, static_cast<int>(T), nh, nkv, hd, ld, static_cast<int>(axes), n[0], n[1], n[2], n[3], interleaved, inverse,
+                                   at.stream);
     }), op);
     return Py_NewRef(a[0]);
 }
@@ -247,8 +258,11 @@ PyObject* window_fwd(PyObject* const* a) {
     need(c.hd % 8 == 0, op, "needs a head dimension of a multiple of 8");
     Piece both_of(c.rows * width * 2 + c.rows * c.nh * 4);
     const at::Tensor out = both_of.make(at::kBFloat16, {c.rows, width}), lse = both_of.make(at::kFloat, {c.B, c.nh, c.S});
+    const void* qkvp = p(qkv);
+    void* outp = p(out);
+    float* lsep = p<float>(lse);
     launched(without_gil([&] {
-        return cai_flash_attn_window_fwd(p(qkv), ld, p(out), p<float>(lse), c.B, c.S, c.nh, c.nkv, c.hd, c.scale, c.window, c.sinks, at.stream);
+        return cai_flash_attn_window_fwd(qkvp, ld, outp, lsep, c.B, c.S, c.nh, c.nkv, c.hd, c.scale, c.window, c.sinks, at.stream);
     }), op);
     THPObjectPtr both(PyTuple_New(2));
     if (!both) throw Raised();
@@ -283,9 +297,12 @@ PyObject* window_bwd(PyObject* const* a) {
     const at::Tensor made = dqkv ? at::Tensor() : make(at, at::kBFloat16, {c.rows, c.cols});
     Piece work((scratch ? 0 : bytes) + (delta ? 0 : stats * 4));
     const at::Tensor parts = scratch ? *scratch : bytes ? work.make(at::kByte, {bytes}) : at::Tensor(), sums = delta ? *delta : work.make(at::kFloat, {stats});
+    const void *qkvp = p(qkv), *outp = p(out), *doutp = p(dout);
+    const float* lsep = p<float>(lse);
+    float* sumsp = p<float>(sums);
+    void *dqkvp = dqkv ? p(*dqkv) : p(made), *partsp = p(parts);
     launched(without_gil([&] {
-        return cai_flash_attn_window_bwd(p(qkv), ld, p(out), p(dout), p<float>(lse), p<float>(sums), dqkv ? p(*dqkv) : p(made), ldq, p(parts), c.B, c.S, c.nh, c.nkv,
-                                         c.hd, c.scale, c.window, c.sinks, at.stream);
+        return cai_flash_attn_window_bwd(qkvp, ld, outp, doutp, lsep, sumsp, dqkvp, ldq, partsp, c.B, c.S, c.nh, c.nkv, c.hd, c.scale, c.window, c.sinks, at.stream);
     }), op);
     return dqkv ? Py_NewRef(a[12]) : THPVariable_Wrap(made);
 }
