@@ -1302,6 +1302,10 @@ CAI_API int cai_flash_attn_window_bwd(const void* qkv, long long ld, const void*
         !window_call_ok("flash_attn_window_bwd (gradient)", dqkv, ldq, dout, B, S, nh, nkv, hd, scale, window, sinks))
         return CAI_K_BAD_ARG;
     if (B == 0 || S == 0) return CAI_K_OK;
+    if (!qkv || !out || !dout || !lse || !delta || !dqkv) {
+        set_last_error("flash_attn_window_bwd: an address is null");
+        return CAI_K_BAD_ARG;
+    }
     if (reinterpret_cast<uintptr_t>(scratch) & 15) {
         set_last_error("flash_attn_window_bwd: the scratch has to start on 16 bytes");
         return CAI_K_BAD_ARG;

@@ -487,6 +487,10 @@ CAI_API int cai_flash_attn_window_fwd(const void* qkv, long long ld, void* out, 
                                       int window, int sinks, void* stream) {
     if (!window_call_ok("flash_attn_window_fwd", qkv, ld, out, B, S, nh, nkv, hd, scale, window, sinks)) return CAI_K_BAD_ARG;
     if (B == 0 || S == 0) return CAI_K_OK;
+    if (!qkv || !out || !lse) {
+        set_last_error("flash_attn_window_fwd: an address is null");
+        return CAI_K_BAD_ARG;
+    }
     CUtensorMap tm;
     if (!encode_tmap_3d(&tm, qkv, static_cast<uint64_t>(nh + 2 * nkv) * hd, S, B, ld, static_cast<uint64_t>(ld) * S, 64, kBlock, 2)) return CAI_K_BAD_ARG;
     WindowFwdParams p;

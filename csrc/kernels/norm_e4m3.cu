@@ -171,6 +171,10 @@ CAI_API int cai_add_rmsnorm_quant(const void* x, long long ldx, const void* resi
         return CAI_K_BAD_ARG;
     }
     if (rows == 0) return CAI_K_OK;
+    if (!x || !g || !q || !scale || !rstd) {
+        set_last_error("add_rmsnorm_quant: an address is null");
+        return CAI_K_BAD_ARG;
+    }
     NormQuantParams p = {};
     p.x = static_cast<const __nv_bfloat16*>(x);
     p.residual = static_cast<const __nv_bfloat16*>(residual);

@@ -138,6 +138,10 @@ CAI_API int cai_rope_apply_axes(void* qkv, const double* freqs, const int* pos, 
         return CAI_K_BAD_ARG;
     }
     if (T == 0 || nh + nkv == 0) return CAI_K_OK;
+    if (!qkv || !freqs || !pos) {
+        set_last_error("rope_apply_axes: an address is null");
+        return CAI_K_BAD_ARG;
+    }
     RopeAxesParams p = {};
     p.qkv = static_cast<__nv_bfloat16*>(qkv);
     p.freqs = freqs; p.pos = pos;

@@ -91,7 +91,11 @@ struct Place {
 };
 Place place(const char* op, std::initializer_list<const at::Tensor*> tensors) {
     for (const at::Tensor* t : tensors)
-        if (t) need(t->is_cuda() && t->layout() == at::kStrided, op, "a tensor is not on the current device");
+        if (t) {
+            need(t->is_cuda() && t->layout() == at::kStrided, op, "a tensor is not on the current device");
+            // Of a wrapper, a fake tensor or one whose storage was given back an address is nothing, or nothing and an offset.
+            need(t->numel() == 0 || (t->has_storage() && t->storage().data()), op, "a tensor has no memory");
+        }
     const c10::DeviceIndex device = c10::cuda::current_device();
     for (const at::Tensor* t : tensors)
         if (t) need(t->get_device() == device, op, "a tensor is not on the current device");

@@ -77,3 +77,64 @@ t = threading.Thread(target=lambda: print("thread"))
 t.start()
 t.join()
 """).splitlines()[-1] == "thread"
+
+
+def test_tensors_without_memory_are_refused(python):
+    """A wrapper's address is 0, or its offset: neither may reach a kernel."""
+    said = python("""
+freqs, pos = Wrapper(64, dtype=torch.float64), Wrapper(1, 4, dtype=torch.int32)
+for offset in (0, 64):
+    qkv, half = Wrapper(4, 512, offset=offset), Wrapper(4, 256, offset=offset)
+    lse, delta, scratch = (Wrapper(*n, dtype=t, offset=offset) for n, t in (((1, 2, 4), torch.float32), ((1, 2, 4), torch.float32), ((1 << 22,), torch.uint8)))
+    print(refused(lambda: ops.rope_apply_axes_(qkv, freqs, pos, 2, 1, 128, (64,))))
+    print(refused(lambda: ops.add_rmsnorm_quant(qkv, qkv, Wrapper(512, offset=offset))))
+    print(refused(lambda: ops.flash_attn_window_fwd(qkv, 1, 4, 2, 1, 128, 4)))
+    print(refused(lambda: ops.flash_attn_window_bwd(qkv, half, half, lse, 1, 4, 2, 1, 128, 4)))
+    print(refused(lambda: ops.flash_attn_window_bwd(qkv, half, half, lse, 1, 4, 2, 1, 128, 4, dqkv=Wrapper(4, 512), delta=delta, scratch=scratch)))
+""").splitlines()
+    assert len(said) == 10 and all("has no memory" in s or "shares memory" in s for s in said), said
+
+
+@pytest.mark.parametrize("missing", ["x", "g", "q", "scale", "rstd"])
+def test_the_norm_launcher_refuses_no_address(missing):
+    from cai_b200.ops import KernelError, calls, check
+    at = dict(x=1 << 20, ldx=256, residual=0, ldr=0, g=1 << 20, h=0, y=0, q=1 << 20, scale=1 << 20, rstd=1 << 20, rows=4, H=256, eps=1e-6, stream=0)
+    at[missing] = 0
+    with pytest.raises(KernelError, match="add_rmsnorm_quant: .*null"):
+        check(calls().cai_add_rmsnorm_quant(*at.values()), "norm")
+    at["rows"] = 0
+    assert calls().cai_add_rmsnorm_quant(*at.values()) == 0
+
+
+@pytest.mark.parametrize("missing", ["qkv", "freqs", "pos"])
+def test_the_rotation_launcher_refuses_no_address(missing):
+    from cai_b200.ops import KernelError, calls, check
+    at = dict(qkv=1 << 20, freqs=1 << 20, pos=1 << 20, ldp=10, T=10, nh=2, nkv=1, hd=128, ld=512, axes=1, n0=64, n1=0, n2=0, n3=0, interleaved=0, inverse=0, stream=0)
+    at[missing] = 0
+    with pytest.raises(KernelError, match="rope_apply_axes: .*null"):
+        check(calls().cai_rope_apply_axes(*at.values()), "rope")
+    at["T"] = 0
+    assert calls().cai_rope_apply_axes(*at.values()) == 0
+
+
+@pytest.mark.parametrize("missing", ["qkv", "out", "lse"])
+def test_the_window_forward_launcher_refuses_no_address(missing):
+    from cai_b200.ops import KernelError, calls, check
+    at = dict(qkv=1 << 20, ld=512, out=1 << 20, lse=1 << 20, B=1, S=256, nh=2, nkv=1, hd=128, scale=0.1, window=64, sinks=4, stream=0)
+    at[missing] = 0
+    with pytest.raises(KernelError, match="flash_attn_window_fwd: .*null"):
+        check(calls().cai_flash_attn_window_fwd(*at.values()), "window")
+    at["S"] = 0
+    assert calls().cai_flash_attn_window_fwd(*at.values()) == 0
+
+
+@pytest.mark.parametrize("missing", ["qkv", "out", "dout", "lse", "delta", "dqkv"])
+def test_the_window_backward_launcher_refuses_no_address(missing):
+    from cai_b200.ops import KernelError, calls, check
+    at = dict(qkv=1 << 20, ld=512, out=1 << 20, dout=1 << 20, lse=1 << 20, delta=1 << 20, dqkv=1 << 20, ldq=512, scratch=1 << 20, B=1, S=256, nh=2, nkv=1, hd=128, scale=0.1,
+              window=64, sinks=4, stream=0)
+    at[missing] = 0
+    with pytest.raises(KernelError, match="flash_attn_window_bwd: .*null"):
+        check(calls().cai_flash_attn_window_bwd(*at.values()), "window")
+    at["B"] = 0
+    assert calls().cai_flash_attn_window_bwd(*at.values()) == 0
