@@ -1000,38 +1000,122 @@ int configure_bwd(int dev) {
 }
 
 // ---------------------------------------------------------------------------- the windowed form's row sums
-// sum_d dO O has the rounding of O in it, and dS = P (dP - delta) is a difference: where a query sees few keys, what O was rounded by counts for more than what dS is (of two
-// keys dq and dk were off by 2.5 roundings, of sixteen by 1.55, of a hundred by 1.48, 1.41 being P's or dS's and the result's own). So there delta is sum_j P dP,
-// which it stands for, in fp32: a warp takes sixteen queries of a head and eight keys at a time, with the warp's own matrix instruction (a tile of 128 x 128 would be
-// seen to an eighth and less). The order of the head's dimension inside a product is free: a lane takes eight of them in a row, of queries and of keys.
-// kFewKeys: seen by a query at most; kFewRows: of a sequence, whose early queries see few whatever the window is. In small grids the four warps of a CTA share the keys of one
-// piece (`ways`): the time is one warp's chain of loads and exponentials. us of a backward, so / from O: 4 x 4096 tokens, 16 / 8 heads, window 8 239 / 216, 3 x 1000, 9 / 3 heads,
-// window 20 33.4 / 30.4 (four ways 37.8), 96 tokens, 8 / 2 heads 12.1 / 10.4 (one way 16.0).
-constexpr int kFewKeys = 24, kFewRows = 96;
+// sum_d dO O has the rounding of O in it, and dS = P (dP - delta) is a difference: where a query sees few keys, what O was rounded by counts for more than what dS is. In
+// roundings of the result, 1.41 being P's or dS's and the result's own, dq of a sequence's rows 0-5 was off by 1.8-2.1, of rows 6-15 by 1.6, of rows 32 on by 1.45-1.5.
+// So delta of such rows is sum_j P dP, which it stands for, in fp32: of the first kFewRows of every sequence, and of all where the window and the sinks are no more than kFewKeys keys.
+// dq is off by 1.3-1.5 then, wherever the row lies. A warp takes sixteen queries of a head and eight keys at a time, with the warp's own matrix instruction (a tile of
+// 128 x 128 would be seen to an eighth and less). The order of the head's dimension inside a product is free: a lane takes eight of them in a row, of queries and of keys.
+// In small grids the four warps of a CTA share the keys of one piece (`ways`): the time is one warp's chain of loads and exponentials (96 tokens, 8 / 2 heads, all rows so: 12.1 us a
+// backward, one way 16.0). The other rows' sums are CTAs of the same launch, so that the chain is hidden behind their bytes: with the first 32 rows so, and from O alone, us
+// of a backward: 2 x 128 tokens, 2 / 1 heads 10.1 / 9.7, 333, 8 / 1 heads 14.8 / 14.4, 8 x 128, 8 / 2 heads 14.7 / 14.2, 16 x 256, 16 / 4 heads 48.5 / 47.2, 4 x 4096, 16 / 8 heads
+// the same within its noise of 1 %. With the first 96 rows so 17.4, 18.5 and 54 for the second to fourth. Three CTAs an SM: four of 128 registers spill (333 tokens: 16.4).
+constexpr int kFewKeys = 24, kFewRows = 32;      // kFewRows: those that see up to kFewKeys, in whole pieces of sixteen
 __device__ __forceinline__ void mma_16x8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__global__ void __launch_bounds__(128, 4)
-attn_window_row_sums_kernel(const __nv_bfloat16* __restrict__ qkv, long long ld, const __nv_bfloat16* __restrict__ dout, const float* __restrict__ lse,
-                            float* __restrict__ delta, int B, int S, int nh, int nkv, float scale_log2, AttnWindow win, int ways) {
+// The other rows', from O: those from `first` on of each sequence, walked as one array, eight times kUnroll of them a CTA. Sixteen lanes a row as in attn_delta_kernel; a warp
+// that has eight pairs of rows adds them up together: a lane gives half of its sums away at each of the first steps.
+template <int kUnroll>
+__device__ __forceinline__ void window_row_sums_of_out(const __nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ dout, float* __restrict__ delta, int B, int S,
+                                                       int nh, int first, unsigned cta) {
+    const unsigned each = static_cast<unsigned>(S - first) * nh, total = each * B, skip = static_cast<unsigned>(first) * nh;
+    const unsigned w0 = cta * (8u * kUnroll) + (threadIdx.x >> 4);
+    const int sub = threadIdx.x & 15;
+    uint4 a[kUnroll], d[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+        const unsigned w = w0 + 8u * i;
+        a[i] = d[i] = make_uint4(0, 0, 0, 0);
+        if (w < total) {
+            const size_t off = static_cast<size_t>(w + (w / each + 1) * skip) * kAttnHD + sub * 8;
+            a[i] = *reinterpret_cast<const uint4*>(out + off);
+            d[i] = *reinterpret_cast<const uint4*>(dout + off);
+        }
+    }
+    float s[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+        uint64_t s2 = 0;
+        const uint32_t x[4] = {a[i].x, a[i].y, a[i].z, a[i].w}, y[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s2 = fma2(pair_of(bf16_lo(x[k]), bf16_hi(x[k])), pair_of(bf16_lo(y[k]), bf16_hi(y[k])), s2);
+        const float2 v = floats_of(s2);
+        s[i] = v.x + v.y;
+    }
+    // the lane's row of the kUnroll: bit by bit, as it gives the others away
+    unsigned mine = 0;
+    int o = 8;
+#pragma unroll
+    for (int half = kUnroll / 2; half > 0; half /= 2, o >>= 1) {
+        const bool up = sub & o;
+        mine += up ? half : 0;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+            const float keep = up ? s[i + half] : s[i], give = up ? s[i] : s[i + half];
+            s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+    }
+    const int rest = o;
+#pragma unroll
+    for (; o > 0; o >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+    const unsigned w = w0 + 8u * mine;
+    if (!(sub & (2 * rest - 1)) && w < total) {
+        const unsigned b = w / each, in = w - b * each, at = in / nh, h = in - at * nh;
+        delta[(static_cast<size_t>(b) * nh + h) * S + first + at] = s[0];
+    }
+}
+__global__ void __launch_bounds__(128, 3)
+attn_window_row_sums_kernel(const __nv_bfloat16* __restrict__ qkv, long long ld, const __nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ dout,
+                            const float* __restrict__ lse, float* __restrict__ delta, int B, int S, int nh, int nkv, float scale_log2, AttnWindow win, int exact,
+                            int ways, unsigned exact_ctas, int unroll) {
     __shared__ float sums[4][16];
     grid_dep_begin();
+    if (blockIdx.x >= exact_ctas) {
+        if (unroll == 8) window_row_sums_of_out<8>(out, dout, delta, B, S, nh, exact, blockIdx.x - exact_ctas);
+        else window_row_sums_of_out<2>(out, dout, delta, B, S, nh, exact, blockIdx.x - exact_ctas);
+        return;
+    }
     // heads fastest: those of a kv head read the same keys
-    const int pieces = (S + 15) / 16, lane = threadIdx.x & 31, row = lane >> 2, part = lane & 3;
+    const int pieces = (exact + 15) / 16, lane = threadIdx.x & 31, row = lane >> 2, part = lane & 3;
     const int warp = threadIdx.x >> 5, mine = ways == 4 ? warp : 0;
-    const long long item = ways == 4 ? blockIdx.x : static_cast<long long>(blockIdx.x) * 4 + warp;
-    if (item >= static_cast<long long>(pieces) * nh * B) return;
-    const int h = static_cast<int>(item % nh), q0 = static_cast<int>(item / nh % pieces) * 16, b = static_cast<int>(item / nh / pieces), g = h / (nh / nkv);
+    const unsigned item = ways == 4 ? blockIdx.x : blockIdx.x * 4 + warp;      // the rows of all heads fit 30 bits
+    if (item >= static_cast<unsigned>(pieces) * nh * B) return;
+    const unsigned piece = item / nh;
+    const int h = item - piece * nh, b = piece / pieces, q0 = (piece - b * pieces) * 16, g = h / (nh / nkv);
     const long long first = static_cast<long long>(b) * S;
+    const int reach = q0 - win.window + 1, near = (reach > 0 ? reach : 0) & ~7, last = q0 + 15 < S - 1 ? q0 + 15 : S - 1;
+    const int sinks = win.sinks < near ? win.sinks : near;
+    // eight keys at a time, of the sinks and from `near` on; the first of them are asked for with the queries
+    uint4 kk[4], vv[4];
+    auto fetch = [&](int k0) {
+        const int at = k0 + row;
+        const __nv_bfloat16* k = qkv + (first + at) * ld + (nh + g) * kAttnHD + part * 8;
+        const __nv_bfloat16* v = k + nkv * kAttnHD;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            kk[c] = vv[c] = make_uint4(0, 0, 0, 0);
+            if (at < S) {
+                kk[c] = *reinterpret_cast<const uint4*>(k + c * 32);
+                vv[c] = *reinterpret_cast<const uint4*>(v + c * 32);
+            }
+        }
+    };
+    const int step = ways * 8;
+    auto behind = [&](int k0) {      // the keys after these
+        const int k1 = k0 + step;
+        return k0 < near && k1 >= sinks ? near + mine * 8 : k1;
+    };
+    int k0 = mine * 8 < sinks ? mine * 8 : near + mine * 8;
+    if (k0 <= last) fetch(k0);
     uint4 q[2][4], d[2][4];
-    float neg_lse2[2], sum[2] = {0.f, 0.f};
+    float lse_at[2], sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int at = q0 + row + u * 8;
         const bool there = at < S;
-        neg_lse2[u] = there ? lse[(static_cast<long long>(b) * nh + h) * S + at] * -1.4426950408889634f : -INFINITY;
+        lse_at[u] = there ? lse[(static_cast<long long>(b) * nh + h) * S + at] : INFINITY;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             q[u][c] = d[u][c] = make_uint4(0, 0, 0, 0);
@@ -1041,20 +1125,8 @@ attn_window_row_sums_kernel(const __nv_bfloat16* __restrict__ qkv, long long ld,
             }
         }
     }
-    auto keys = [&](int k0) {
-        const int at = k0 + row;
+    while (k0 <= last) {
         float s[4] = {}, dp[4] = {};
-        const __nv_bfloat16* k = qkv + (first + at) * ld + (nh + g) * kAttnHD + part * 8;
-        const __nv_bfloat16* v = k + nkv * kAttnHD;
-        uint4 kk[4], vv[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            kk[c] = vv[c] = make_uint4(0, 0, 0, 0);
-            if (at < S) {
-                kk[c] = *reinterpret_cast<const uint4*>(k + c * 32);
-                vv[c] = *reinterpret_cast<const uint4*>(v + c * 32);
-            }
-        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             mma_16x8(s, q[0][c].x, q[1][c].x, q[0][c].y, q[1][c].y, kk[c].x, kk[c].y);
@@ -1062,22 +1134,22 @@ attn_window_row_sums_kernel(const __nv_bfloat16* __restrict__ qkv, long long ld,
             mma_16x8(dp, d[0][c].x, d[1][c].x, d[0][c].y, d[1][c].y, vv[c].x, vv[c].y);
             mma_16x8(dp, d[0][c].z, d[1][c].z, d[0][c].w, d[1][c].w, vv[c].z, vv[c].w);
         }
+        const int now = k0;
+        k0 = behind(k0);
+        if (k0 <= last) fetch(k0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int i = q0 + row + (e >> 1) * 8, j = k0 + part * 2 + (e & 1);
-            if (j <= i && (j > i - win.window || j < win.sinks)) sum[e >> 1] += fast_exp2(s[e] * scale_log2 + neg_lse2[e >> 1]) * dp[e];
+            const int i = q0 + row + (e >> 1) * 8, j = now + part * 2 + (e & 1);
+            if (j <= i && (j > i - win.window || j < win.sinks))
+                sum[e >> 1] += fast_exp2(s[e] * scale_log2 - lse_at[e >> 1] * 1.4426950408889634f) * dp[e];
         }
-    };
-    const int reach = q0 - win.window + 1, near = (reach > 0 ? reach : 0) & ~7, last = q0 + 15 < S - 1 ? q0 + 15 : S - 1;
-    const int sinks = win.sinks < near ? win.sinks : near;
-    for (int k0 = mine * 8; k0 < sinks; k0 += ways * 8) keys(k0);
-    for (int k0 = near + mine * 8; k0 <= last; k0 += ways * 8) keys(k0);
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 1);
         sum[u] += __shfl_xor_sync(0xffffffffu, sum[u], 2);
     }
-    float* out = delta + (static_cast<long long>(b) * nh + h) * S + q0;
+    float* to = delta + (static_cast<long long>(b) * nh + h) * S + q0;
     if (ways == 4) {
         if (part == 0) {
             sums[warp][row] = sum[0];
@@ -1085,10 +1157,10 @@ attn_window_row_sums_kernel(const __nv_bfloat16* __restrict__ qkv, long long ld,
         }
         __syncthreads();
         if (threadIdx.x < 16 && q0 + threadIdx.x < S)
-            out[threadIdx.x] = sums[0][threadIdx.x] + sums[1][threadIdx.x] + sums[2][threadIdx.x] + sums[3][threadIdx.x];
+            to[threadIdx.x] = sums[0][threadIdx.x] + sums[1][threadIdx.x] + sums[2][threadIdx.x] + sums[3][threadIdx.x];
     } else if (part == 0) {
-        if (q0 + row < S) out[row] = sum[0];
-        if (q0 + row + 8 < S) out[row + 8] = sum[1];
+        if (q0 + row < S) to[row] = sum[0];
+        if (q0 + row + 8 < S) to[row + 8] = sum[1];
     }
 }
 
@@ -1335,19 +1407,18 @@ CAI_API int cai_flash_attn_window_bwd(const void* qkv, long long ld, const void*
         set_last_error("flash_attn_window_bwd: needs the scratch that cai_flash_attn_window_bwd_scratch says");
         return CAI_K_BAD_ARG;
     }
-    const long long rows = static_cast<long long>(B) * S * nh;
-    cudaError_t e;
-    if (S <= kFewRows || static_cast<long long>(p.win.window) + p.win.sinks <= kFewKeys) {
-        const long long pieces = static_cast<long long>((S + 15) / 16) * nh * B;
-        const int ways = pieces < 4 * sm_count(dev) ? 4 : 1;
-        e = launch_early(attn_window_row_sums_kernel, static_cast<unsigned>((pieces * ways + 3) / 4), 128, 0, st, static_cast<const __nv_bfloat16*>(qkv), ld,
-                         static_cast<const __nv_bfloat16*>(dout), lse, delta, B, S, nh, nkv, p.scale_log2, p.win, ways);
-    } else {
-        constexpr unsigned per_cta = 16u * kDeltaUnroll;
-        e = launch_early(attn_delta_kernel, static_cast<unsigned>((rows + per_cta - 1) / per_cta), 256, 0, st,
-                         static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(dout), delta, static_cast<unsigned>(rows),
-                         static_cast<unsigned>(S), static_cast<unsigned>(nh), true, static_cast<unsigned int*>(nullptr), 0u);
-    }
+    // rows below `exact` of each sequence from P and dP, the others from O
+    const int exact = static_cast<long long>(p.win.window) + p.win.sinks <= kFewKeys || S < kFewRows ? S : kFewRows;
+    const long long pieces = static_cast<long long>((exact + 15) / 16) * nh * B;
+    const long long others = static_cast<long long>(S - exact) * nh * B;
+    // Four ways where that leaves the other rows' CTAs beside them (16 x 256 tokens, 16 / 4 heads, whose 512 pieces would come first: 49.9 us, one way 48.5); of the
+    // others few rows a CTA only where all CTAs are one wave (8 x 128, 8 / 2 heads: 15.5, eight a thread 15.0 with the four ways).
+    const int sms = sm_count(dev), ways = pieces < (others ? 1 : 4) * sms ? 4 : 1, exact_ctas = static_cast<int>((pieces * ways + 3) / 4);
+    const int unroll = others < 2 * 16 * sms ? 2 : 8;
+    const int other_ctas = static_cast<int>((others + 8 * unroll - 1) / (8 * unroll));
+    cudaError_t e = launch_early(attn_window_row_sums_kernel, exact_ctas + other_ctas, 128, 0, st, static_cast<const __nv_bfloat16*>(qkv), ld,
+                                 static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(dout), lse, delta, B, S, nh, nkv, p.scale_log2, p.win, exact,
+                                 ways, static_cast<unsigned>(exact_ctas), unroll);
     const int kv_ctas = p.cut.near_ctas + p.cut.far_ctas;
     const long long q_ctas = static_cast<long long>((S + kAttnTile - 1) / kAttnTile) * nh * B;
     if (e == cudaSuccess)

@@ -361,3 +361,18 @@ def test_tensors_elsewhere_are_refused():
         ops.flash_attn_window_fwd(qkv.cpu(), 1, 8, 2, 1, HD, 4)
     with pytest.raises(ops.KernelError, match="current device"):
         ops.flash_attn_window_bwd(qkv, out, dout.cpu(), lse, 1, 8, 2, 1, HD, 4)
+
+
+@pytest.mark.parametrize("B,S,nh,nkv,window,sinks", [(2, 97, 8, 2, 97, 0), (1, 256, 8, 2, 200, 4), (3, 700, 4, 4, 64, 30), (1, 3000, 8, 1, 1024, 4), (4, 513, 4, 2, 513, 0), (2, 1200, 8, 4, 20, 5)])
+def test_early_rows_of_long_sequences_are_no_less_exact(B, S, nh, nkv, window, sinks):
+    """The first queries of a sequence see few keys, however long it is and whatever the window: their dq alone, within what test_few_visible_keys_are_no_less_exact
+    asks of whole tensors. (A query behind the first 24 of these shapes sees at least 25.)"""
+    from cai_b200 import ops
+    qkv, dout = _inputs(B, S, nh, nkv, 23)
+    out, lse = ops.flash_attn_window_fwd(qkv, B, S, nh, nkv, HD, window, sinks)
+    dqkv = ops.flash_attn_window_bwd(qkv, out, dout, lse, B, S, nh, nkv, HD, window, sinks)
+    d = _reference(qkv, dout, B, S, nh, nkv, window, sinks, HD ** -0.5)[3]
+    got, want = (t.double().view(B, S, -1)[:, :24, :nh * HD] for t in (dqkv, d))
+    for rows in (slice(0, 6), slice(6, 24), slice(0, 24)):
+        once = (want[:, rows].to(torch.bfloat16).double() - want[:, rows]).norm()
+        assert (got[:, rows] - want[:, rows]).norm() <= 1.6 * once
