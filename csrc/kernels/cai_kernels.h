@@ -275,12 +275,12 @@ CAI_API int cai_flash_attn_window_fwd(const void* qkv, long long ld, void* out, 
 CAI_API long long cai_flash_attn_window_bwd_scratch(int B, int S, int nh, int nkv, int window, int sinks);
 /* The blocks of 64 keys that query tile i (128 rows) of the forward kernel takes, in order, two ints a block: its number, and how many of its keys the products take.
  * And the items that CTA `cta` of `ctas` of it takes, in order, three ints an item: query tile, head, sequence. Return their numbers, of which
- * `capacity` are written. Need no GPU. */
+ * `capacity` are written; 0 for what no launch takes. Need no GPU. */
 CAI_API int cai_flash_attn_window_blocks(int S, int window, int sinks, int i, int* blocks, int capacity);
 CAI_API int cai_flash_attn_window_items(int B, int S, int nh, int ctas, int cta, int* items, int capacity);
 /* What the CTAs of its dK / dV part work on, on `sms` SMs, eight ints a CTA: key tile, batch, kv head, first query head, query heads, first query tile, query
  * tiles (none or less: nothing), slot of 128 KB of the scratch (-1: none). Returns their number, of which `capacity` are written. And the key tiles
- * that query tile i of its dQ part takes, in order, with how many of their keys the products take. Need no GPU. */
+ * that query tile i of its dQ part takes, in order, with how many of their keys the products take. 0 for what no launch takes. Need no GPU. */
 CAI_API int cai_flash_attn_window_walk(int B, int S, int nh, int nkv, int window, int sinks, int sms, int* parts, int capacity);
 CAI_API int cai_flash_attn_window_keys(int S, int window, int sinks, int i, int* tiles, int capacity);
 CAI_API int cai_flash_attn_window_bwd(const void* qkv, long long ld, const void* out, const void* dout, const float* lse, float* delta, void* dqkv,

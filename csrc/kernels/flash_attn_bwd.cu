@@ -1341,6 +1341,7 @@ CAI_API int cai_flash_attn_bwd_rope(const void* qkv, const void* out, const void
 }
 
 CAI_API int cai_flash_attn_window_walk(int B, int S, int nh, int nkv, int window, int sinks, int sms, int* parts, int capacity) {
+    if (!window_sizes_ok(B, S, nh, nkv, window, sinks) || sms <= 0) return 0;
     const AttnWindow w = {window < S ? window : S, sinks < S ? sinks : S};
     const AttnWindowParts c = window_parts(w, B, S, nh, nkv, sms);
     const int n = c.near_ctas + c.far_ctas;
@@ -1352,6 +1353,7 @@ CAI_API int cai_flash_attn_window_walk(int B, int S, int nh, int nkv, int window
     return n;
 }
 CAI_API int cai_flash_attn_window_keys(int S, int window, int sinks, int i, int* tiles, int capacity) {
+    if (!window_sizes_ok(1, S, 1, 1, window, sinks) || i < 0 || i > (S - 1) / kAttnTile) return 0;
     const WindowKeys keys({window < S ? window : S, sinks < S ? sinks : S}, i);
     for (int k = 0; k < keys.n && k < capacity; ++k) {
         tiles[2 * k] = keys.tile(k);
@@ -1361,7 +1363,7 @@ CAI_API int cai_flash_attn_window_keys(int S, int window, int sinks, int i, int*
 }
 
 CAI_API long long cai_flash_attn_window_bwd_scratch(int B, int S, int nh, int nkv, int window, int sinks) {
-    if (B <= 0 || S <= 0 || nkv <= 0 || nh < nkv || nh % nkv || window < 1 || sinks < 0) return 0;
+    if (!window_sizes_ok(B, S, nh, nkv, window, sinks)) return 0;
     const int sms = sm_count(current_device());
     const AttnWindowParts c = window_parts({window < S ? window : S, sinks < S ? sinks : S}, B, S, nh, nkv, sms > 0 ? sms : 148);
     return (static_cast<long long>(c.near_slots) + c.far_ctas) * 131072;

@@ -458,6 +458,7 @@ attn_window_fwd_kernel(const __grid_constant__ CUtensorMap tm, const WindowFwdPa
 using namespace cai;
 
 CAI_API int cai_flash_attn_window_blocks(int S, int window, int sinks, int i, int* blocks, int capacity) {
+    if (!window_sizes_ok(1, S, 1, 1, window, sinks) || i < 0 || i > (S - 1) / kAttnTile) return 0;
     const AttnWindow w = {window < S ? window : S, sinks < S ? sinks : S};
     const WindowBlocks b(w, i, S);
     for (int k = 0; k < b.n && k < capacity; ++k) {
@@ -467,6 +468,7 @@ CAI_API int cai_flash_attn_window_blocks(int S, int window, int sinks, int i, in
     return b.n;
 }
 CAI_API int cai_flash_attn_window_items(int B, int S, int nh, int ctas, int cta, int* items, int capacity) {
+    if (!window_sizes_ok(B, S, nh, nh, 1, 0) || cta < 0 || cta >= ctas) return 0;
     const int tiles = (S + kAttnTile - 1) / kAttnTile, all = tiles * nh * B;
     const Divisor heads_all(nh * B), heads(nh);
     int n = 0;

@@ -122,6 +122,10 @@ bool encode_tmap_3d(CUtensorMap* out, const void* base, uint64_t cols, uint64_t 
     return true;
 }
 
+bool window_sizes_ok(int B, int S, int nh, int nkv, int window, int sinks) {
+    return B > 0 && S > 0 && nkv > 0 && nh > 0 && nh % nkv == 0 && B <= 65535 && nh <= 65535 && static_cast<long long>(B) * S * nh <= 0x3fffffffll && window >= 1 && sinks >= 0;
+}
+
 bool window_call_ok(const char* name, const void* qkv, long long ld, const void* out, int B, int S, int nh, int nkv, int hd, float scale, int window, int sinks) {
     if (hd != 128 || nkv <= 0 || nh <= 0 || nh % nkv || B < 0 || S < 0) {
         set_last_error("%s: needs head_dim 128 and heads %% kv_heads == 0 (hd=%d, %d heads, %d kv heads, B=%d, S=%d)", name, hd, nh, nkv, B, S);

@@ -57,6 +57,8 @@ inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, dim3 block
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Args&&>(args)...);
 }
 
+// Sizes that windowed attention has tiles, items and parts for: all of them are counted in 32 bits.
+bool window_sizes_ok(int B, int S, int nh, int nkv, int window, int sinks);
 // The arguments that both directions of windowed attention have in common; says what is wrong with them.
 bool window_call_ok(const char* name, const void* qkv, long long ld, const void* out, int B, int S, int nh, int nkv, int hd, float scale, int window, int sinks);
 

@@ -306,3 +306,23 @@ def test_frequencies():
     f = ops.rope_freqs(128, 500000.0, device="cpu")
     assert f.dtype == torch.float64 and f.shape == (64,) and f[0] == 1.0
     assert abs(f[32].item() - 500000.0 ** -0.5) < 1e-15
+
+
+def test_lists_of_what_is_refused_are_empty():
+    """The lists of tiles, items and parts, and the scratch, of sizes that no launch takes: in a process of its own, since a division by zero or a list without an end would be
+    this one's."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    cases = [("items", a) for a in ((0, 300, 2, 8, 0), (1, 0, 2, 8, 0), (1, 300, 0, 8, 0), (1, 300, 2, 0, 0), (1, 300, 2, 8, -1), (1, 300, 2, 8, 8), (60000, 60000, 2, 8, 0))]
+    cases += [(c, a) for c in ("blocks", "keys") for a in ((0, 4, 1, 0), (300, 0, 1, 0), (300, 4, -1, 0), (300, 4, 1, 3), (300, 4, 1, -1))]
+    for sizes in ((0, 300, 2, 1, 4, 1), (1, 0, 2, 1, 4, 1), (1, 300, 2, 0, 4, 1), (1, 300, 1, 2, 4, 1), (1, 300, 3, 2, 4, 1), (1, 300, 2, 1, 0, 1), (1, 300, 2, 1, 4, -1),
+                  (60000, 60000, 2, 1, 4, 1)):
+        cases += [("walk", sizes + (148,)), ("bwd_scratch", sizes)]
+    cases.append(("walk", (1, 300, 2, 1, 4, 1, 0)))
+    code = "from cai_b200.ops import lib\n"
+    for name, args in cases:
+        args = ", ".join(map(str, args + (() if name == "bwd_scratch" else (None, 0))))
+        code += f"got = lib().cai_flash_attn_window_{name}({args}); assert got == 0, ('{name}', {args}, got)\n"
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=Path(__file__).resolve().parent.parent)
+    assert done.returncode == 0, (done.returncode, done.stderr[-500:])
