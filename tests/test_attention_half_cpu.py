@@ -326,3 +326,13 @@ def test_lists_of_what_is_refused_are_empty():
         code += f"got = lib().cai_flash_attn_window_{name}({args}); assert got == 0, ('{name}', {args}, got)\n"
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=Path(__file__).resolve().parent.parent)
     assert done.returncode == 0, (done.returncode, done.stderr[-500:])
+
+
+@pytest.mark.parametrize("change", [dict(B=65536, S=1), dict(nh=65536, ld=65538 * 128, ldq=65538 * 128), dict(B=32768, S=32768, nh=2)], ids=str)
+def test_refusals_of_sizes_say_the_limits(change):
+    """The limits as the docstring has them."""
+    from cai_b200 import ops
+    assert "65535 sequences" in ops.flash_attn_window_fwd.__doc__ and "65535 heads" in ops.flash_attn_window_fwd.__doc__
+    for name in ("fwd", "bwd"):
+        with pytest.raises(ops.KernelError, match="65535 sequences, 65535 heads and 2\\^30 rows"):
+            ops.check(getattr(ops.calls(), f"cai_flash_attn_window_{name}")(*_window(name, **change)), "flash_attn_window")
