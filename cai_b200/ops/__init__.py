@@ -283,7 +283,7 @@ def flash_attn_bwd(qkv, out, dout, lse, B, S, nh, nkv, hd, scale=None, dqkv=None
 def flash_attn_window_fwd(qkv, B, S, nh, nkv, hd, window, sinks=0, scale=None):
     """Causal GQA flash attention with a window and sinks over packed ``qkv`` ``[B*S, (nh + 2 nkv) * hd]`` (bf16, any row pitch that is a multiple of 8): query i
     sees key j if ``j <= i`` and (``j > i - window`` or ``j < sinks``). Any ``S``; ``window >= 1``, ``sinks >= 0``, head_dim 128; up to 65535 sequences, 65535 heads and
-    2^30 rows of all heads (``B * S * nh``). Returns ``out`` bf16 ``[B*S, nh * hd]`` and ``lse`` f32 ``[B, nh, S]``, which share an allocation. All of ``qkv`` has to be
+    fewer than 2^30 rows of all heads (``B * S * nh``). Returns ``out`` bf16 ``[B*S, nh * hd]`` and ``lse`` f32 ``[B, nh, S]``, which share an allocation. All of ``qkv`` has to be
     finite: a value that is not reaches queries of its tile that do not see it, though not another sequence."""
     return native().flash_attn_window_fwd(qkv, B, S, nh, nkv, hd, window, sinks, scale)
 

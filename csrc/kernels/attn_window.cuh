@@ -1,4 +1,4 @@
-// attn_window.cuh - what windowed attention's forward and backward kernels share: which tiles belong together, tiles of one sequence, arithmetic on pairs.
+// attn_window.cuh - what windowed attention's forward and backward kernels share: which tiles belong together, what is seen of them.
 #pragma once
 
 #include "attn_common.cuh"
@@ -41,12 +41,6 @@ __host__ __device__ inline int window_last_query_tile(const AttnWindow& w, int j
 // Is something hidden between query tile i and key tile j <= i?
 __device__ __forceinline__ bool window_masks(const AttnWindow& w, int i, int j) {
     return i == j || ((i - j + 1) * kAttnTile > w.window && (j + 1) * kAttnTile > w.sinks);
-}
-
-// A tile of one sequence of a packed tensor, 128 columns from x on, in two 64-column sub-tiles. Rows past the sequence's end come as zeros.
-__device__ __forceinline__ void load_seq_tile(void* dst, const CUtensorMap* tm, uint64_t* bar, int x, int row, int b) {
-    tma_load_3d(dst, tm, bar, x, row, b);
-    tma_load_3d(static_cast<uint8_t*>(dst) + kAttnSub, tm, bar, x + 64, row, b);
 }
 
 }  // namespace cai

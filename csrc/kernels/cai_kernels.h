@@ -264,7 +264,7 @@ CAI_API int cai_flash_attn_bwd_rope(const void* qkv, const void* out, const void
                                     const float* table, int B, int S, int nh, int nkv, int hd, float scale, int parts, void* stream);
 
 /* ---- the same with a window and sinks, over sequences of any length: query i sees key j if j <= i and (j > i - window or j < sinks). window >= 1, so
- * that every row sees itself; sinks >= 0; up to 65535 sequences, 65535 heads and 2^30 rows of all heads. qkv and dqkv have row pitches ld and ldq (multiples of 8 elements); out, dout [B*S, nh*hd] and lse, delta
+ * that every row sees itself; sinks >= 0; up to 65535 sequences, 65535 heads and fewer than 2^30 rows of all heads. qkv and dqkv have row pitches ld and ldq (multiples of 8 elements); out, dout [B*S, nh*hd] and lse, delta
  * [B, nh, S] are dense. Rows of 16-byte alignment, head_dim 128. Nothing is read or written past a sequence's last row. Values have to be finite: a
  * hidden key has weight 0, and 0 times what is not finite is not 0. */
 CAI_API int cai_flash_attn_window_fwd(const void* qkv, long long ld, void* out, float* lse, int B, int S, int nh, int nkv, int hd, float scale,

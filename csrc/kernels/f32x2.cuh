@@ -30,10 +30,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-__device__ __forceinline__ uint64_t neg2(uint64_t a) {
-    const float2 v = floats_of(a);
-    return pair_of(-v.x, -v.y);
-}
 // The largest of three.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;

@@ -118,7 +118,6 @@ struct WindowStream : WindowTile {
     WindowBlocks keys;
     __device__ WindowStream(const WindowFwdParams& p) : round(-1), u(0) { keys.n = 0; next_item(p); }
     __device__ bool there() const { return keys.n > 0; }
-    __device__ bool first() const { return u == 0; }
     __device__ bool last() const { return u + 1 == keys.n; }
     __device__ int row() const { return keys.block(u) * kBlock; }
     __device__ void next_item(const WindowFwdParams& p) {

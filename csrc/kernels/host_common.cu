@@ -142,7 +142,7 @@ bool window_call_ok(const char* name, const void* qkv, long long ld, const void*
     // rows and columns are counted in 32 bits; up to 65535 sequences and heads, which is the interface's limit (no grid needs it: they all go along x)
     const long long rows = static_cast<long long>(B) * S, cols = (static_cast<long long>(nh) + 2ll * nkv) * hd;
     if (rows * nh > 0x3fffffffll || S > 0x7fffffff - 256 || cols > 0x7fffffffll || B > 65535 || nh > 65535) {
-        set_last_error("%s: up to 65535 sequences, 65535 heads and 2^30 rows of all heads (B=%d, S=%d, %d heads)", name, B, S, nh);
+        set_last_error("%s: up to 65535 sequences, 65535 heads and fewer than 2^30 rows of all heads (B=%d, S=%d, %d heads)", name, B, S, nh);
         return false;
     }
     if (ld < cols || (ld & 7) || (reinterpret_cast<uintptr_t>(qkv) & 15) || (reinterpret_cast<uintptr_t>(out) & 15)) {

@@ -334,5 +334,5 @@ def test_refusals_of_sizes_say_the_limits(change):
     from cai_b200 import ops
     assert "65535 sequences" in ops.flash_attn_window_fwd.__doc__ and "65535 heads" in ops.flash_attn_window_fwd.__doc__
     for name in ("fwd", "bwd"):
-        with pytest.raises(ops.KernelError, match="65535 sequences, 65535 heads and 2\\^30 rows"):
+        with pytest.raises(ops.KernelError, match="65535 sequences, 65535 heads and fewer than 2\\^30 rows"):
             ops.check(getattr(ops.calls(), f"cai_flash_attn_window_{name}")(*_window(name, **change)), "flash_attn_window")
