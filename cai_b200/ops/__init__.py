@@ -174,8 +174,8 @@ def add_rmsnorm_quant(x, residual, g, eps=1e-6, *, keep_y=False):
 
     ``x`` and ``residual`` are bf16 ``[rows, H]`` of any row pitch that is a multiple of 8, ``H`` a multiple of 128 up to 16384; ``g`` bf16 ``[H]``. Returns
     ``(h, q, s, rstd, y)``: ``h`` bf16 (``x`` itself where ``residual`` is None), ``q`` e4m3 ``[rows, H]``, ``s`` f32 ``[rows, H / 128]``, ``rstd`` f32
-    ``[rows]``, ``y`` bf16, or None without ``keep_y`` (a weight gradient reads it); h, y and rstd share an allocation, q and s another. ``q`` is rounded once,
-    from y in fp32. The gradients are
+    ``[rows]``, ``y`` bf16, or None without ``keep_y`` (a weight gradient reads it); h, y and rstd share an allocation, q and s another. ``q`` is rounded to
+    e4m3 once, from y in fp32 times the reciprocal of ``s``. The gradients are
     ``rmsnorm_bwd(h, g, rstd, dy, dx=dh, dx_accumulate=True)``: ``dh``, the gradient of ``h`` that comes past the norm, becomes that of x and of residual."""
     return native().add_rmsnorm_quant(x, residual, g, eps, keep_y)
 

@@ -168,7 +168,8 @@ CAI_API int cai_rmsnorm_bwd_rounds(int rows, int H, int ctas, int cta, int lost_
 
 /* RMSNorm in front of a block-scaled e4m3 product, with the residual's addition: h = bf16(x + residual) (residual null: h = x),
  * rstd = (mean(h^2) + eps)^(-1/2), y = h * rstd * g, scale[row, b] = max |y| of columns 128 b .. 128 b + 127 / 448 (1 where they are all zero,
- * otherwise at least 2^-100 / 448), q = e4m3(y / scale), rounded once. x and residual have pitches ldx and ldr (elements, multiples of 8; h may be x or residual where their pitch is H);
+ * otherwise at least 2^-100 / 448), q = e4m3(y / scale), rounded to e4m3 once, from y
+ * in f32 times the reciprocal of the scale. x and residual have pitches ldx and ldr (elements, multiples of 8; h may be x or residual where their pitch is H);
  * h, y [rows, H] bf16 (either may be null), q [rows, H] e4m3, scale [rows, H / 128] and rstd [rows] f32. H % 128 == 0, H <= 16384, every row on 16
  * bytes. The backward pass is cai_rmsnorm_bwd on h with dx_accumulate: dx holds the gradient of h that comes past the norm, and ends as that of
  * x and of the residual. No counterpart in the reference. */

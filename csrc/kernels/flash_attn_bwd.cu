@@ -40,8 +40,9 @@
 // tiles that a query tile sees. It cuts dK / dV's sums into parts that a third kernel adds up in a fixed order (AttnWindowParts): over heads and query tiles in small
 // grids, and the sinks' sums, which run over all later queries. Tensor maps with the sequences apart bring rows past a sequence's end as zeros and leave them out of the
 // result. Warps that see nothing of a tile skip its exponentials. us: 4 x 4096 tokens, 16 / 8 heads, 4 sinks, window 1024 540 in a burst, 590 back to back at the power
-// limit (985 W, 1657-1725 MHz; 560 TFLOP/s of the five products of what is seen; seven are computed), window 128 280; 16384 tokens, window 4096 1680; 333 tokens, 8 / 1 heads 14.4, 2 x 128,
-// 2 / 1 heads 9.7. dQ from the same scores as dK / dV, added to in L2 in a fixed order, took 725 against 600: the additions go at some 30 bytes a cycle and SM.
+// limit (985 W, 1657-1725 MHz; 560 TFLOP/s of the five products of what is seen; seven are computed), window 128 280; 16384 tokens, window 4096 1680; 333 tokens, 8 / 1 heads 14.8, 2 x 128,
+// 2 / 1 heads 10.1. (Window 128 moves 62 us of bytes: a CTA has two to four steps there, and set-up, first loads, staging and writing, which take longer, overlap nothing: it has
+// the SM's whole shared memory.) dQ from the same scores as dK / dV, added to in L2 in a fixed order, took 725 against 600: the additions go at some 30 bytes a cycle and SM.
 //
 // Replaces the reference's one-thread-per-query backward, which recomputes dp twice, scatters
 // dK/dV with atomicAdd and never zeroes dq/dk/dv (src/cuda/cai_kernels.cu:110-143).
@@ -564,7 +565,8 @@ __device__ __forceinline__ void attn_dkdv(const CUtensorMap& tm_qkv, const CUten
                 const int from = (j - i) * kAttnTile + r - qb;
                 seen = ~bits_below(from) & (j * kAttnTile + r < p.win.sinks ? ~0u : bits_below(from + p.win.window));
             }
-            // Of a tile at either end of the window six of sixteen warps see nothing, of a sinks' tile behind it at least twelve: zeros, for no exponentials.
+            // Of a tile at either end of the window six of sixteen warps see nothing, of a sinks' tile behind it all but four for each 32 sinks begun: zeros, for no
+            // exponentials.
             const bool none = kWindow && diag && !__any_sync(0xffffffffu, seen);
             const float delta = delta_next;
             if (!mbar_wait_warp(s_full, it & 1, abort_flag, p.status, CAI_DEV_TIMEOUT_ATTN)) { ok = false; break; }
@@ -1006,7 +1008,7 @@ int configure_bwd(int dev) {
 // dq is off by 1.3-1.5 then, wherever the row lies. A warp takes sixteen queries of a head and eight keys at a time, with the warp's own matrix instruction (a tile of
 // 128 x 128 would be seen to an eighth and less). The order of the head's dimension inside a product is free: a lane takes eight of them in a row, of queries and of keys.
 // In small grids the four warps of a CTA share the keys of one piece (`ways`): the time is one warp's chain of loads and exponentials (96 tokens, 8 / 2 heads, all rows so: 12.1 us a
-// backward, one way 16.0). The other rows' sums are CTAs of the same launch, so that the chain is hidden behind their bytes: with the first 32 rows so, and from O alone, us
+// backward, one way 16.0; all rows so and from O alone, 4 x 4096, 16 / 8 heads, window 8 239 / 216, 3 x 1000, 9 / 3 heads, window 20 33.4 / 30.4, four ways 37.8). The other rows' sums are CTAs of the same launch, so that the chain is hidden behind their bytes: with the first 32 rows so, and from O alone, us
 // of a backward: 2 x 128 tokens, 2 / 1 heads 10.1 / 9.7, 333, 8 / 1 heads 14.8 / 14.4, 8 x 128, 8 / 2 heads 14.7 / 14.2, 16 x 256, 16 / 4 heads 48.5 / 47.2, 4 x 4096, 16 / 8 heads
 // the same within its noise of 1 %. With the first 96 rows so 17.4, 18.5 and 54 for the second to fourth. Three CTAs an SM: four of 128 registers spill (333 tokens: 16.4).
 constexpr int kFewKeys = 24, kFewRows = 32;      // kFewRows: those that see up to kFewKeys, in whole pieces of sixteen

@@ -2,7 +2,7 @@
 //
 //   s_ij = scale q_i . k_j where j <= i and (j > i - window or j < sinks), else -inf;   o_i = sum_j softmax(s_i)_j v_j;   lse_i = log sum_j exp(s_ij)
 //
-// One pass over the keys of a 128-row query tile, 64 at a time, with a running maximum and sum. Two CTAs share an SM (112 KB and half of the tensor memory each) and stay
+// One pass over the keys of a 128-row query tile, 64 at a time, with a running maximum and sum. Two CTAs share an SM (105 KB and half of the tensor memory each) and stay
 // for the whole launch: each takes one (query tile, head, sequence) after the other, and the blocks of all of them are one stream, so that loads and scores
 // run ahead over the end of a tile; with windows of few blocks a tile's beginning and end are most of it. Warp 0 loads by TMA, warp 1 issues the tcgen05
 // products, warps 2-5 are the softmax, a thread a row. S = Q K^T lies in tensor memory for two blocks, so that the next block's scores are there

@@ -3,10 +3,10 @@
 //   h = bf16(x + residual)     rstd = (mean(h^2) + eps)^(-1/2)     y = h * rstd * g
 //   s[row, b] = max |y| of the row's 128 columns b / 448 (1 where they are all zero)     q = e4m3(y / s)
 //
-// The norm is that of the rounded h, which is what the backward pass reads; q is rounded once, from y in fp32 (through a bf16 y, as the two kernels of
+// The norm is that of the rounded h, which is what the backward pass reads; q is rounded to e4m3 once, from y in fp32 times the reciprocal of s (through a bf16 y, as the two kernels of
 // their own do it, values next to a border of e4m3 are rounded twice).
-// Measured on a B200: 16384 x 4096 with residual and y 89 us (9 bytes an element, 6.8 TB/s: the rate of a copy), without either 48 (3 bytes, 4.2 TB/s, bound by
-// instructions), 8192 x 2048 24.7, 1777 x 1408 without either 3.8, 256 x 256 1.8, where a launch's own latencies are all there is.
+// Measured on a B200: 16384 x 4096 with residual and y 89 us (9 bytes an element, 6.8 TB/s: the rate of a copy), without either 48 (3 bytes, 4.2 TB/s:
+// issue slots 69 % busy, DRAM 42 %; a CTA loads its rows and then computes, so that the two alternate, and each row reads and unpacks the gain anew), 8192 x 2048 24.7, 1777 x 1408 without either 3.8, 256 x 256 1.8, where a launch's own latencies are all there is.
 #include <cuda_fp8.h>
 
 #include "cai_kernels.h"
@@ -33,7 +33,7 @@ __device__ __forceinline__ uint64_t bf16x2_pair(uint32_t v) { return pair_of(bf1
 __device__ __forceinline__ float block_scale(float amax) { return amax > 0.f ? fmaxf(amax, 0x1p-100f) / 448.f : 1.f; }
 
 // A row is shared by p.warps warps, each lane holding kChunks times eight of its columns in registers, 256 columns of a warp apart: sixteen lanes hold one
-// block of the quantiser. A CTA takes blockDim / (32 * p.warps) rows. With the residual and y this is bound by its 9 bytes an element, without them, 3 bytes, by
+// block of the quantiser. A CTA takes blockDim / (32 * p.warps) rows. With the residual and y this is bound by its 9 bytes an element, without them, 3 bytes, more by
 // its instructions: hence the arithmetic on pairs, and (kChunks = 4) the four blocks' maxima reduced together: a lane that gives two of its
 // four away at the first step and one at the second is left with one, whose scale and reciprocal it computes for the sixteen.
 template <int kChunks>
